@@ -30,7 +30,7 @@ enum { UNIMP_ACT_NONE = 0, UNIMP_ACT_GELU = 1, UNIMP_ACT_QUICKGELU = 2, UNIMP_AC
 enum { UNIMP_MASK_NONE = 0, UNIMP_MASK_CAUSAL = 1, UNIMP_MASK_SEGMENT = 2 };
 
 int unimp_abi_version(void);
-int unimp_struct_size(int which);            /* sizeof(unimp_gemm_desc / unimp_attn_desc / unimp_image_desc / unimp_mx_gemm_desc / unimp_decode_step_desc) for which = 0 ... 4 */
+int unimp_struct_size(int which);            /* sizeof(unimp_gemm_desc / unimp_attn_desc / unimp_image_desc / unimp_mx_gemm_desc / unimp_decode_step_desc / unimp_kv4_attn_desc) for which = 0 ... 5 */
 const char* unimp_last_error(void);          /* thread-local, valid until the next failing call */
 /* internal helpers shared by the translation units (exported for the tests' benefit only) */
 int unimp_set_error(int code, const char* msg);
@@ -438,6 +438,58 @@ typedef struct unimp_image_desc {
 int unimp_image_resize_normalize(const uint8_t* src, const unimp_image_desc* descs, int n_images, int max_h,
                                  const int32_t* tables, uint8_t* tmp, int out_h, int out_w, const float* mean,
                                  const float* std, void* out, int out_f32, uint8_t* out_u8, void* stream);
+
+/* ---- paged K/V cache held in 4 bits (decode; eval_rec.py:100-110, eval_exp.py:103-113, eval_img_gen.py:102-111 through Flamingo.generate) -----
+ * A page holds 32 tokens of one head of one layer, keys and values, as MX blocks: e2m1 codes with one E8M0 scale byte per (token, 32 consecutive dims; the
+ * last block of a head dim of 80 is 16 wide): 2^e, e = max(floor(log2 of the block's largest magnitude) - 2, -125), codes rounded to nearest even, saturated at
+ * 6; a block that holds an infinity or a NaN is stored as scale 255 and reads back as NaN.  unimp_kv4_page_bytes(hd) = 32 hd + 64 ceil(hd / 32) bytes (head dims 64, 80,
+ * 128; -1: any other) against 128 hd in bf16.  Byte layout: unimp_amd/csrc/kv4.h.  A pool is [n_pages][heads][page bytes] per layer, 16-byte aligned;
+ * SLOT s = token s % 32 of page s / 32.  A row's pages are named by its row of an int32 table: column c = tokens 32 c ... 32 c + 31.
+ * Slots and page ids outside the pool are never accessed: such a token is not written, reads as zero and is not attended to.  Pages need no initial contents. */
+int unimp_kv4_page_bytes(int hd);
+/* quantise k, v (bf16; element strides: token, head; unit dim stride) of `tokens` tokens into their slots.  Different tokens of one page may be written by different
+ * calls or rows in any order; the same slot twice in one call holds one of the two. */
+int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, void* pages, int64_t n_pages, int heads, int hd,
+                    const int64_t* slots, int64_t tokens, void* stream);
+/* a decode step's tokens: rotate q and k of every row (half-split pairs, row r with ITS table row; rot = 0: none), write q (bf16, rounded once) to q_out
+ * [rows][heads][hd] and quantise the rotated k and v into slot slots[r].  Operand layout of unimp_decode_rope_append; qkv is not modified.  The rotation is computed in
+ * 64 bits from the fp32 tables. */
+int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,
+                          const float* cos_rows, const float* sin_rows, void* q_out, void* pages, int64_t n_pages, const int64_t* slots, void* stream);
+/* the values held (exact in bf16): k, v [layers][tokens][heads][hd]; layer_stride in bytes between the pools of two layers */
+int unimp_kv4_read(const void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, const int64_t* slots, int64_t tokens, void* k, void* v,
+                   void* stream);
+/* page tables [rows][width] and slots from the rows' lengths, one launch, no host value.  Row r has cached[r] tokens, fresh[r] arrive, its pages have to reach cover[r]
+ * tokens (NULL: cached + fresh): need = min(width, ceil(max(cover, cached + fresh) / 32)) columns of which the first mapped[r] are there already.  In a group
+ * (rows g group ... : the beams of a prompt) the rows after the first take the first row's pages for the columns below alias = min(shared_len[g] / 32, need, the first
+ * row's columns).  The other new columns take free_pages[cursor + i] in row order (none left: -1).  Written: the new columns of tables; mapped_out[r]; *cursor_out (above
+ * n_free: that many pages were missing); cu[rows + 1], the first packed index of every row's new tokens; slots[max_tokens], the slot of every new token in packed
+ * order, -1 behind the last one and for a token without a page.  mapped_out and cursor_out must not be the inputs. */
+int unimp_page_tables_extend(int32_t* tables, int rows, int width, const int32_t* mapped, const int32_t* cached, const int32_t* fresh, const int32_t* cover,
+                             const int32_t* free_pages, int n_free, const int32_t* cursor, int group, const int32_t* shared_len, int32_t* mapped_out,
+                             int32_t* cursor_out, int64_t* slots, int64_t max_tokens, int32_t* cu, void* stream);
+/* beam search (transformers' _reorder_cache on the paged cache): row j of group g goes on with the hypothesis of row src_local[g group + j] of its group (out of range:
+ * its own).  pos[g group] tokens are cached.  The table columns below pos / 32 are taken over from the source row (full pages are shared by name, nothing is copied);
+ * the page of column pos / 32, if it holds tokens, is copied for all layers into the row's own.  The rows' pages of that column must be different; group <= 16. */
+int unimp_kv4_reorder_beams(void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, int32_t* tables, int width, int group, int n_groups,
+                            const int64_t* src_local, const int64_t* pos, void* stream);
+/* attention of ONE query token per row over its cached tokens j < min(lens[r], 32 width): softmax_j(scale q k_j + alibi_slopes[h] j) v_j; a row without tokens gives
+ * zeros.  q [rows][heads][hd] views, heads a multiple of kv_heads (at most 16 query heads to a key head; query head h reads key head h / (heads / kv_heads)).
+ * group > 1 with shared_len (int32 [rows / group]): the rows of a group name the same pages in the columns below shared_len[g] / 32; with group * heads / kv_heads <= 16 those
+ * pages are read once per group.  The tokens of a (row, key head) are split over workgroups; partial (max, sum, o[hd]) in fp32 go to `workspace`
+ * (unimp_kv4_attn_workspace floats; NULL when that is 0) and are merged in a fixed order: no atomics, the same bits at every launch, capturable. */
+typedef struct {
+  const void* q; int64_t q_row_stride, q_head_stride;
+  const void* pages; int64_t n_pages; int kv_heads, hd;
+  const int32_t* tables; int64_t table_stride; int width;
+  const int32_t* lens;
+  int rows, heads;
+  float scale; const float* alibi_slopes;
+  void* out; int64_t o_row_stride, o_head_stride;
+  int group; const int32_t* shared_len;
+} unimp_kv4_attn_desc;
+int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc* d);
+int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* workspace, void* stream);
 
 #ifdef __cplusplus
 }

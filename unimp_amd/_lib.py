@@ -43,6 +43,13 @@ class AttnDesc(C.Structure):
                                                     ("q_row_off", c_p), ("q_len", c_p), ("k_row_off", c_p), ("flags", c_i)]
 
 
+class Kv4AttnDesc(C.Structure):
+    """include/unimp_hip.h unimp_kv4_attn_desc"""
+    _fields_ = [("q", c_p), ("q_row_stride", c_l), ("q_head_stride", c_l), ("pages", c_p), ("n_pages", c_l), ("kv_heads", c_i), ("hd", c_i),
+                ("tables", c_p), ("table_stride", c_l), ("width", c_i), ("lens", c_p), ("rows", c_i), ("heads", c_i), ("scale", c_f), ("alibi_slopes", c_p),
+                ("out", c_p), ("o_row_stride", c_l), ("o_head_stride", c_l), ("group", c_i), ("shared_len", c_p)]
+
+
 class MxGemmDesc(C.Structure):
     _fields_ = [("A", c_p), ("B", c_p), ("scale_a", c_p), ("scale_b", c_p), ("C", c_p),
                 ("bias", c_p), ("res", c_p), ("aux", c_p), ("pre", c_p)] + \
@@ -105,6 +112,14 @@ _SIGS = {
     "unimp_focal_ce_bwd_rows": [c_p, c_l, c_p, c_p, c_f, c_i, c_p, c_p, c_p, c_p, c_p, c_i, c_p, c_l, c_i, c_i, c_p],
     "unimp_sumsq_bf16": [c_p, c_l, c_p, c_p],
     "unimp_adamw_flat": [c_p, c_p, c_p, c_p, c_p, c_l, c_l, c_f, c_f, c_f, c_f, c_f, c_i, c_p, c_f, c_f, c_i, c_p],
+    "unimp_kv4_page_bytes": [c_i],
+    "unimp_kv4_write": [c_p, c_p, c_l, c_l, c_l, c_l, c_p, c_l, c_i, c_i, c_p, c_l, c_p],
+    "unimp_kv4_rope_append": [c_p, c_l, c_l, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p, c_p, c_p, c_l, c_p, c_p],
+    "unimp_kv4_read": [c_p, c_l, c_i, c_l, c_i, c_i, c_p, c_l, c_p, c_p, c_p],
+    "unimp_page_tables_extend": [c_p, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_p, c_p, c_p, c_l, c_p, c_p],
+    "unimp_kv4_reorder_beams": [c_p, c_l, c_i, c_l, c_i, c_i, c_p, c_i, c_i, c_i, c_p, c_p, c_p],
+    "unimp_kv4_attn_workspace": [C.POINTER(Kv4AttnDesc)],
+    "unimp_kv4_attn_decode": [C.POINTER(Kv4AttnDesc), c_p, c_p],
     "unimp_image_resize_normalize": [c_p, c_p, c_i, c_i, c_p, c_p, c_i, c_i, c_p, c_p, c_p, c_i, c_p, c_p],
 }
 
@@ -136,12 +151,13 @@ def lib():
             fn.argtypes, fn.restype = args, c_i
         L.unimp_embedding_bwd_sorted_scratch.restype = c_l
         L.unimp_beam_topk_scratch.restype = c_l
+        L.unimp_kv4_attn_workspace.restype = c_l
         if L.unimp_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.unimp_abi_version()}, this package binds version {ABI_VERSION} -- a stale build; "
                               "rebuild with `make -C unimp_amd/csrc`")
         # the descriptors are passed by pointer: a layout the library and these ctypes mirrors disagree on would bind silently
         L.unimp_struct_size.restype, L.unimp_struct_size.argtypes = c_i, [c_i]
-        for which, st in ((0, GemmDesc), (1, AttnDesc), (3, MxGemmDesc), (4, DecodeStepDesc)):
+        for which, st in ((0, GemmDesc), (1, AttnDesc), (3, MxGemmDesc), (4, DecodeStepDesc), (5, Kv4AttnDesc)):
             if L.unimp_struct_size(which) != C.sizeof(st):
                 raise ImportError(f"{LIB_PATH}: sizeof descriptor {which} is {L.unimp_struct_size(which)} in the library, "
                                   f"{C.sizeof(st)} in {st.__name__} -- stale build")

@@ -21,7 +21,7 @@ extern "C" int unimp_check_launch(const char* what) {
   return UNIMP_OK;
 }
 
-// sizeof of the descriptor structs, so a binding can verify its mirror of them (0: gemm, 1: attention, 2: image, 3: MX gemm, 4: decode step)
+// sizeof of the descriptor structs, so a binding can verify its mirror of them (0: gemm, 1: attention, 2: image, 3: MX gemm, 4: decode step, 5: 4-bit page attention)
 extern "C" int unimp_struct_size(int which) {
   switch (which) {
     case 0: return (int)sizeof(unimp_gemm_desc);
@@ -29,6 +29,7 @@ extern "C" int unimp_struct_size(int which) {
     case 2: return (int)sizeof(unimp_image_desc);
     case 3: return (int)sizeof(unimp_mx_gemm_desc);
     case 4: return (int)sizeof(unimp_decode_step_desc);
+    case 5: return (int)sizeof(unimp_kv4_attn_desc);
     default: return -1;
   }
 }

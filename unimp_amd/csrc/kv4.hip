@@ -1,0 +1,372 @@
+// Paged 4-bit K/V cache of a decode (F1: the past_key_values behind Flamingo.generate, eval_rec.py:100-110, eval_exp.py:103-113, eval_img_gen.py:102-111):
+// quantise-and-write of prompt tokens, rotary embedding + append of a decode step's tokens, read-back as values, page tables and slots from the rows' lengths,
+// and the beam reorder.  Layout of a page: kv4.h.  Attention over the pages: kv4_attn.hip.
+//
+// An MX block of x: e = max(floor(log2 max |x|) - 2, -125), codes rne(x / 2^e) on e2m1, saturated at 6: 2^e code is exact in bf16, so what is read back is
+// exactly what the attention multiplies.  All of these are bound by bytes; the arithmetic is a few instructions per element.
+#include <type_traits>
+#include "kv4.h"
+#include "unimp_hip.h"
+
+template <typename F> static int kv4_for_hd(int hd, F f) {
+  switch (hd) {
+    case 64: return f(std::integral_constant<int, 64>());
+    case 80: return f(std::integral_constant<int, 80>());
+    case 128: return f(std::integral_constant<int, 128>());
+    default: return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
+  }
+}
+extern "C" int unimp_kv4_page_bytes(int hd) { return hd == 64 || hd == 80 || hd == 128 ? 32 * hd + 64 * ((hd + 31) / 32) : -1; }
+
+// ------------------------------------------------------------------------------------------- write
+// A RUN is a maximal stretch of consecutive rows whose slots are consecutive inside one page; a workgroup (chunk of 32 rows, head) owns the runs that START
+// in its chunk (a run has at most 32 rows: it looks 31 rows ahead), so every row is read once, by one workgroup, whatever the alignment of the rows to the
+// pages.  A V dword holds 8 tokens of one dim: the codes of a run turn round in LDS and a dword whose 8 tokens are all in the run is stored; the dwords at
+// the ragged ends of a run change their nibbles by atomic and + or (another workgroup may hold the other nibbles; the fields are disjoint, the result does not
+// depend on the order).
+template <int D>
+__global__ __launch_bounds__(256) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
+                                                        uint8_t* __restrict__ pages, long n_pages, int heads, const int64_t* __restrict__ slots, long tokens) {
+  using P = Kv4<D>;
+  __shared__ int64_t sl[65];
+  __shared__ uint8_t vc[32][D + 4];
+  const int tid = threadIdx.x, head = blockIdx.y;
+  const long i0 = (long)blockIdx.x * 32;
+  if (tid < 65) {
+    const long i = i0 - 1 + tid;
+    const int64_t s = i >= 0 && i < tokens ? slots[i] : -1;
+    sl[tid] = s >= 0 && s < n_pages * KV4_PAGE ? s : -1;
+  }
+  __syncthreads();
+  for (int a = 0; a < 32;) {                                        // rows i0 + a: uniform over the workgroup
+    const int64_t s0 = sl[a + 1];
+    const bool starts = s0 >= 0 && (sl[a] < 0 || sl[a] + 1 != s0 || (s0 & 31) == 0);
+    if (!starts) { ++a; continue; }                                 // no slot, or the tail of the previous chunk's last run
+    int n = 1;
+    const int t0 = (int)(s0 & 31);
+    while (t0 + n < 32 && a + n < 64 && sl[a + 1 + n] == s0 + n) ++n;
+    uint8_t* page = pages + ((s0 >> 5) * heads + head) * (long)P::BYTES;
+    const bool is_v = tid >= 128;
+    const int w = tid & 127, t = w / P::NB, b = w - t * P::NB;      // (token, block): 32 NB <= 128
+    if (t < n) {
+      const bf16* x = (is_v ? v + (i0 + a + t) * v_ts + head * v_hs : k + (i0 + a + t) * k_ts + head * k_hs) + 32 * b;
+      const int nd = b == P::NB - 1 ? P::BLK_LAST : 32;
+      float f[32];
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        bf16x8 u = {};
+        if (8 * c < nd) u = *(const bf16x8*)(x + 8 * c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { f[8 * c + j] = bf2f(u[j]); m = max(m, __float_as_uint(f[8 * c + j]) & 0x7fffffffu); }
+      }
+      const int sb = kv4_scale_byte((int)(m >> 23));
+      const float scale = __uint_as_float((uint32_t)(sb == 255 ? 127 : sb) << 23);
+      uint32_t q[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r = 0;
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c], f[8 * c + 1], scale, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 2], f[8 * c + 3], scale, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 4], f[8 * c + 5], scale, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 6], f[8 * c + 7], scale, 3);
+        q[c] = sb == 255 ? 0u : r;
+      }
+      if (!is_v) {
+        uint8_t* o = page + P::k_byte(t0 + t, b);
+        *(u32x2*)o = u32x2{q[0], q[1]};
+        if (nd == 32) *(u32x2*)(o + 8) = u32x2{q[2], q[3]};
+        page[P::ks_byte(t0 + t, b)] = (uint8_t)sb;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) if (j < nd) vc[t0 + t][32 * b + j] = (uint8_t)((q[j >> 3] >> (4 * (j & 7))) & 15u);
+        page[P::vs_byte(t0 + t, b)] = (uint8_t)sb;
+      }
+    }
+    __syncthreads();
+    for (int w2 = tid; w2 < 4 * D; w2 += 256) {
+      const int g = w2 / D, x = w2 - g * D, d = (x / P::NI) + 16 * (x % P::NI);
+      uint32_t val = 0, mask = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int tt = 16 * (j >> 2) + 4 * g + (j & 3);
+        if (tt >= t0 && tt < t0 + n) { val |= (uint32_t)vc[tt][d] << (4 * j); mask |= 15u << (4 * j); }
+      }
+      uint32_t* o = (uint32_t*)(page + P::VOFF) + w2;
+      if (mask == 0xffffffffu) *o = val;
+      else if (mask) { atomicAnd(o, ~mask); atomicOr(o, val); }
+    }
+    __syncthreads();
+    a += n;
+  }
+}
+
+extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, void* pages, int64_t n_pages, int heads,
+                               int hd, const int64_t* slots, int64_t tokens, void* stream) {
+  if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
+  if (tokens <= 0 || heads <= 0 || n_pages <= 0) return UNIMP_OK;
+  if (heads > 65535 || tokens > (int64_t)1 << 28) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^28 tokens");
+  if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
+    return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_write: strides multiples of 8 elements, 16-byte aligned pointers");
+  return kv4_for_hd(hd, [&](auto d) {
+    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32), heads), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
+                       (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, slots, (long)tokens);
+    return unimp_check_launch("kv4_write");
+  });
+}
+
+// ------------------------------------------------------------------------------------------- decode step: rotary embedding + append
+// Block (row, head): thread d holds dim d of q, k and v.  The rotation runs in 64 bits (two products of a bf16 and an fp32, exact there): a code is decided
+// next to a border, and k's codes are those of the exact rotation of the given tables.  The nibbles of V go in by atomics: two rows of a launch may write
+// different tokens of one page.
+__device__ __forceinline__ uint32_t kv4_code_f64(double x, double inv) {
+  const double a = fabs(x) * inv;
+  const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
+  return c | (x < 0.0 ? 8u : 0u);
+}
+template <int D>
+__global__ __launch_bounds__(128) void kv4_rope_append_kernel(const bf16* __restrict__ qkv, long row_stride, long head_stride, int q_off, int k_off, int v_off,
+                                                              int rot, const float* __restrict__ cos_rows, const float* __restrict__ sin_rows,
+                                                              bf16* __restrict__ q_out, uint8_t* __restrict__ pages, long n_pages, int heads,
+                                                              const int64_t* __restrict__ slots) {
+  using P = Kv4<D>;
+  const int row = blockIdx.y, head = blockIdx.x, d = threadIdx.x;
+  const bf16* base = qkv + (long)row * row_stride + (long)head * head_stride;
+  double q = 0, k = 0, v = 0;
+  if (d < D) {
+    q = (double)bf2f(base[q_off + d]); k = (double)bf2f(base[k_off + d]); v = (double)bf2f(base[v_off + d]);
+    if (d < rot) {
+      const int h = rot >> 1, i = d < h ? d : d - h, p = d < h ? d + h : d - h;
+      const double c = cos_rows[(long)row * h + i], s = sin_rows[(long)row * h + i];
+      const double q2 = (double)bf2f(base[q_off + p]), k2 = (double)bf2f(base[k_off + p]);
+      q = d < h ? q * c - q2 * s : q * c + q2 * s;
+      k = d < h ? k * c - k2 * s : k * c + k2 * s;
+    }
+    q_out[((long)row * heads + head) * D + d] = f2bf((float)q);
+  }
+  const int64_t slot = slots[row];
+  if (slot < 0 || slot >= n_pages * KV4_PAGE) return;               // uniform over the block
+  const int t = (int)(slot & 31);
+  uint8_t* page = pages + ((slot >> 5) * heads + head) * (long)P::BYTES;
+  uint32_t code[2]; int sb[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const double x = w ? v : k;
+    int e = (int)((__double2hiint(x) >> 20) & 0x7ff);               // exponent field: floor(log2 |x|) + 1023, 2047 for infinity and NaN
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 32));
+    sb[w] = e == 2047 ? 255 : max(e - 1023 - 2, -125) + 127;
+    code[w] = sb[w] == 255 ? 0u : kv4_code_f64(x, __hiloint2double((1023 + 127 - sb[w]) << 20, 0));
+  }
+  uint32_t kk = code[0] << (4 * (d & 7));                           // eight lanes' K codes into one dword
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) kk |= __shfl_xor(kk, o, 8);
+  if (d < D) {
+    if (!(d & 7)) *(uint32_t*)(page + P::k_byte(t, d >> 5) + ((d & 31) >> 1)) = kk;
+    if (!(d & 31)) { page[P::ks_byte(t, d >> 5)] = (uint8_t)sb[0]; page[P::vs_byte(t, d >> 5)] = (uint8_t)sb[1]; }
+    uint32_t* o = (uint32_t*)(page + P::v_dword(t, d));
+    const int sh = 4 * kv4_nibble(t);
+    atomicAnd(o, ~(15u << sh)); atomicOr(o, code[1] << sh);
+  }
+}
+
+extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,
+                                     const float* cos_rows, const float* sin_rows, void* q_out, void* pages, int64_t n_pages, const int64_t* slots, void* stream) {
+  if (!qkv || !q_out || !pages || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
+  if (rows <= 0 || heads <= 0) return UNIMP_OK;
+  if (rot < 0 || (rot & 1) || rot > hd || rows > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_rope_append: rot even and at most the head dim, at most 65535 rows");
+  if ((uintptr_t)pages & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_rope_append: 16-byte aligned pages");
+  return kv4_for_hd(hd, [&](auto d) {
+    hipLaunchKernelGGL((kv4_rope_append_kernel<decltype(d)::value>), dim3(heads, rows), dim3(128), 0, (hipStream_t)stream, (const bf16*)qkv, (long)row_stride,
+                       (long)head_stride, q_off, k_off, v_off, rot, cos_rows, sin_rows, (bf16*)q_out, (uint8_t*)pages, (long)n_pages, heads, slots);
+    return unimp_check_launch("kv4_rope_append");
+  });
+}
+
+// ------------------------------------------------------------------------------------------- read back as values
+template <int D>
+__global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, const int64_t* __restrict__ slots,
+                                                       long tokens, bf16* __restrict__ k, bf16* __restrict__ v) {
+  using P = Kv4<D>;
+  const long per = (long)heads * (D / 8), i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= tokens * per) return;
+  const long tok = i / per; const int r = (int)(i - tok * per), head = r / (D / 8), d = (r - head * (D / 8)) * 8;
+  const int64_t s = slots[tok];
+  bf16x8 ko = {}, vo = {};
+  if (s >= 0 && s < n_pages * KV4_PAGE) {
+    const uint8_t* page = pages + (long)blockIdx.y * layer_stride + ((s >> 5) * heads + head) * (long)P::BYTES;
+    const int t = (int)(s & 31), b = d >> 5, sh = 4 * kv4_nibble(t);
+    const uint32_t kc = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1));
+    const float ks = kv4_scale(page[P::ks_byte(t, b)]), vs = kv4_scale(page[P::vs_byte(t, b)]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ko[j] = f2bf(kv4_value((kc >> (4 * j)) & 15u) * ks);
+      vo[j] = f2bf(kv4_value((*(const uint32_t*)(page + P::v_dword(t, d + j)) >> sh) & 15u) * vs);
+    }
+  }
+  const long o = (((long)blockIdx.y * tokens + tok) * heads + head) * D + d;
+  *(bf16x8*)(k + o) = ko; *(bf16x8*)(v + o) = vo;
+}
+
+extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, const int64_t* slots, int64_t tokens, void* k,
+                              void* v, void* stream) {
+  if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
+  if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
+  if (layers > 65535 || tokens > (int64_t)1 << 28 || tokens * heads * hd > (int64_t)1 << 34)
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and 2^34 elements of a layer");
+  if (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_read: 16-byte aligned pointers");
+  return kv4_for_hd(hd, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens * heads * (D / 8) + 255) / 256), layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
+                       (long)layer_stride, (long)n_pages, heads, slots, (long)tokens, (bf16*)k, (bf16*)v);
+    return unimp_check_launch("kv4_read");
+  });
+}
+
+// ------------------------------------------------------------------------------------------- page tables and slots from lengths
+// One block per row.  What a row takes from the free list starts at the sum of what the rows before it take: every block sums that itself (a handful of
+// integer operations per row, from L2), so the whole step is one launch and nothing is exchanged between blocks.
+struct PageRow { int need, begin; };                                // columns [begin, need) come from the free list
+struct PageArgs {
+  int32_t* tables; const int32_t *mapped, *cached, *fresh, *cover, *free_pages, *cursor, *shared; int32_t *mapped_out, *cursor_out, *cu; int64_t* slots;
+  long max_tokens; int rows, width, n_free, group;
+};
+__device__ __forceinline__ int page_need(const PageArgs& a, int r, int& map) {
+  const long len = (long)max(a.cached[r], 0) + max(a.fresh[r], 0), cov = a.cover ? max((long)a.cover[r], len) : len;
+  map = min(max(a.mapped[r], 0), a.width);
+  return (int)min((cov + KV4_PAGE - 1) / KV4_PAGE, (long)a.width);
+}
+__device__ __forceinline__ PageRow page_row(const PageArgs& a, int r, int& alias, int& map) {
+  const int need = page_need(a, r, map);
+  alias = 0;
+  if (a.shared) {
+    const int g = r / a.group, first = g * a.group;
+    if (r != first) {
+      int m0; const int n0 = page_need(a, first, m0);
+      alias = min(min(max(a.shared[g], 0) / KV4_PAGE, need), max(m0, n0));
+    }
+  }
+  return PageRow{need, max(map, alias)};
+}
+__global__ __launch_bounds__(256) void page_tables_extend_kernel(PageArgs a) {
+  __shared__ long red[3][4];
+  const int r = blockIdx.x, tid = threadIdx.x, first = a.group > 1 ? r / a.group * a.group : r;
+  const bool last = r == a.rows - 1;
+  long before = 0, before_first = 0, tok = 0;
+  for (int i = tid; i < r; i += 256) {
+    int al, m; const PageRow p = page_row(a, i, al, m);
+    const int own = max(p.need - p.begin, 0);
+    before += own; tok += max(a.fresh[i], 0);
+    if (i < first) before_first += own;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { before += __shfl_xor(before, o, 64); before_first += __shfl_xor(before_first, o, 64); tok += __shfl_xor(tok, o, 64); }
+  if (!(tid & 63)) { red[0][tid >> 6] = before; red[1][tid >> 6] = before_first; red[2][tid >> 6] = tok; }
+  __syncthreads();
+  const long cur = a.cursor[0];
+  before = cur + red[0][0] + red[0][1] + red[0][2] + red[0][3];
+  before_first = cur + red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  tok = red[2][0] + red[2][1] + red[2][2] + red[2][3];
+  int alias, map; const PageRow p = page_row(a, r, alias, map);
+  int al0 = 0, map0 = 0, begin0 = 0;
+  if (first != r) begin0 = page_row(a, first, al0, map0).begin;
+  const int32_t* row0 = a.tables + (long)first * a.width;
+  int32_t* row = a.tables + (long)r * a.width;
+  auto from_free = [&](long i) { return i >= 0 && i < a.n_free ? a.free_pages[i] : -1; };
+  auto lookup = [&](int c) {                                         // the row's page of column c < max(map, need) after the call
+    if (c < map) return (int)row[c];
+    if (c < alias) return c < map0 ? (int)row0[c] : from_free(before_first + c - begin0);
+    return c < p.need ? from_free(before + c - p.begin) : -1;
+  };
+  const int n = max(a.fresh[r], 0), have = max(a.cached[r], 0);
+  for (long t = tid; t < n && tok + t < a.max_tokens; t += 256) {
+    const long pos = (long)have + t, c = pos / KV4_PAGE;
+    const long page = c < a.width ? (long)lookup((int)c) : -1;
+    a.slots[tok + t] = page >= 0 ? page * KV4_PAGE + (pos & 31) : -1;
+  }
+  for (int c = map + tid; c < p.need; c += 256) row[c] = lookup(c);
+  if (tid == 0) { a.mapped_out[r] = max(map, p.need); a.cu[r] = (int)tok; }
+  if (last) {
+    if (tid == 0) { a.cu[a.rows] = (int)(tok + n); a.cursor_out[0] = (int)(before + max(p.need - p.begin, 0)); }
+    for (long i = tok + n + tid; i < a.max_tokens; i += 256) a.slots[i] = -1;
+  }
+}
+
+extern "C" int unimp_page_tables_extend(int32_t* tables, int rows, int width, const int32_t* mapped, const int32_t* cached, const int32_t* fresh, const int32_t* cover,
+                                        const int32_t* free_pages, int n_free, const int32_t* cursor, int group, const int32_t* shared_len, int32_t* mapped_out,
+                                        int32_t* cursor_out, int64_t* slots, int64_t max_tokens, int32_t* cu, void* stream) {
+  if (!tables || !mapped || !cached || !fresh || !free_pages || !cursor || !mapped_out || !cursor_out || !cu || (max_tokens > 0 && !slots))
+    return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: null pointer");
+  if (rows <= 0 || width <= 0 || n_free < 0 || max_tokens < 0 || group < 1 || (rows % group))
+    return unimp_set_error(UNIMP_ERR_SHAPE, "page_tables_extend: rows a positive multiple of group, width positive");
+  if (mapped == mapped_out || cursor == cursor_out) return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: the blocks read mapped and cursor throughout; outputs of their own");
+  PageArgs a{tables, mapped, cached, fresh, cover, free_pages, cursor, shared_len, mapped_out, cursor_out, cu, slots, (long)max_tokens, rows, width, n_free, group};
+  hipLaunchKernelGGL(page_tables_extend_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, a);
+  return unimp_check_launch("page_tables_extend");
+}
+
+// ------------------------------------------------------------------------------------------- beam reorder
+// Row j of a group goes on with the hypothesis of row src[j].  Its whole columns (all 32 tokens written) never change again: the table rows take the
+// page ids over, and several rows may name one page.  Only the column that the next token goes to holds a page per row that must be copied; the K pages of a
+// column are enough for ever, since a column's pages stop changing when it is full.  Thread (layer, 16-byte chunk) moves its chunk of all K rows through
+// registers: in place, whatever the permutation.
+template <int KMAX>
+__global__ __launch_bounds__(256) void kv4_reorder_beams_kernel(uint8_t* __restrict__ pages, long layer_stride, long n_pages, long page_stride, int32_t* __restrict__ tables,
+                                                                int width, int K, const int64_t* __restrict__ src, const int64_t* __restrict__ pos) {
+  const int grp = blockIdx.z, tid = threadIdx.x;
+  const int64_t p = pos[(long)grp * K];
+  if (p < 0) return;
+  const long now = p >> 5;
+  int32_t* tab = tables + (long)grp * K * width;
+  int from[KMAX];
+#pragma unroll
+  for (int j = 0; j < KMAX; ++j) {
+    const int64_t s = j < K ? src[(long)grp * K + j] : j;
+    from[j] = s >= 0 && s < K ? (int)s : j;
+  }
+  if (blockIdx.x == gridDim.x - 1) {                                 // the table rows: one block per group
+    if (blockIdx.y) return;
+    for (long c = tid; c < min(now, (long)width); c += 256) {
+      int32_t e[KMAX];
+#pragma unroll
+      for (int j = 0; j < KMAX; ++j) if (j < K) e[j] = tab[(long)from[j] * width + c];
+#pragma unroll
+      for (int j = 0; j < KMAX; ++j) if (j < K) tab[(long)j * width + c] = e[j];
+    }
+    return;
+  }
+  if (!(p & 31) || now >= width) return;                             // nothing in the current page yet
+  const long chunk = ((long)blockIdx.x * 256 + tid) * 16;
+  if (chunk >= page_stride) return;
+  uint8_t* base = pages + (long)blockIdx.y * layer_stride + chunk;
+  u32x4 x[KMAX];
+#pragma unroll
+  for (int j = 0; j < KMAX; ++j) {
+    const int32_t pg = j < K && from[j] != j ? tab[(long)from[j] * width + now] : -1;
+    if (pg >= 0 && pg < n_pages) x[j] = *(const u32x4*)(base + pg * page_stride);
+  }
+#pragma unroll
+  for (int j = 0; j < KMAX; ++j) if (j < K && from[j] != j) {
+    const int32_t pf = tab[(long)from[j] * width + now], pg = tab[(long)j * width + now];
+    if (pf >= 0 && pf < n_pages && pg >= 0 && pg < n_pages) *(u32x4*)(base + pg * page_stride) = x[j];
+  }
+}
+
+extern "C" int unimp_kv4_reorder_beams(void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, int32_t* tables, int width, int group,
+                                       int n_groups, const int64_t* src_local, const int64_t* pos, void* stream) {
+  if (!pages || !tables || !src_local || !pos) return unimp_set_error(UNIMP_ERR_ARG, "kv4_reorder_beams: null pointer");
+  const int pb = unimp_kv4_page_bytes(hd);
+  if (pb < 0) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
+  if (layers <= 0 || n_groups <= 0 || group <= 1 || width <= 0) return UNIMP_OK;
+  if (group > 16 || layers > 65535 || n_groups > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_reorder_beams: at most 16 beams, 65535 layers and groups");
+  if (((uintptr_t)pages | layer_stride) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_reorder_beams: 16-byte aligned pages and layer stride");
+  const long stride = (long)heads * pb;
+  dim3 grid((unsigned)((stride / 16 + 255) / 256 + 1), layers, n_groups);
+#define KV4_REORDER(KM) hipLaunchKernelGGL((kv4_reorder_beams_kernel<KM>), grid, dim3(256), 0, (hipStream_t)stream, (uint8_t*)pages, (long)layer_stride, (long)n_pages, \
+                                           stride, tables, width, group, src_local, pos)
+  if (group <= 4) KV4_REORDER(4);
+  else if (group <= 8) KV4_REORDER(8);
+  else KV4_REORDER(16);
+#undef KV4_REORDER
+  return unimp_check_launch("kv4_reorder_beams");
+}

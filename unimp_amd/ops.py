@@ -1069,3 +1069,167 @@ def gemm_mx(a, b, *, bias=None, act=None, pre=None, aux=None, res=None, out=None
         epi = "+".join(n for n, t in (("bias", bias), ("act", act), ("pre", pre), ("aux", aux), ("res", res)) if t is not None) or "plain"
         GEMM_PROFILE.append((e0, e1, 2.0 * M * N * K, (M, N, K, epi + ("->mx" if out_mx else ""), 0, "mxfp8")))
     return MxTensor(out, sc_out) if out_mx else out
+
+
+# ----------------------------------------------------------------------------------------------- paged K/V cache held in 4 bits (decode)
+KV4_PAGE = 32                                                 # tokens of a page
+
+
+def kv4_page_bytes(hd):
+    """bytes of one page (32 tokens of one head of one layer, keys and values) at head dim 64, 80 or 128"""
+    if hd not in (64, 80, 128):
+        raise ValueError(f"the 4-bit cache serves head dims 64, 80 and 128, not {hd}")
+    return 32 * hd + 64 * ((hd + 31) // 32)
+
+
+def _same_device(*ts):
+    """every given tensor on one HIP device, and that device current: a launch goes to the current device's stream"""
+    dev = _dev(ts[0]).device
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise _lib.UnimpHipError(f"tensors on {dev} and {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise _lib.UnimpHipError(f"tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _kv4_pool(pages, hd, layered=False):
+    """checks a pool [(layers,) n_pages, heads, page bytes] -> (layers, byte stride between layers, n_pages, heads)"""
+    pb = kv4_page_bytes(hd)
+    _need(pages.dtype == torch.uint8 and pages.dim() in ((3, 4) if layered else (3,)) and pages.shape[-1] == pb and pages.stride()[-3:] == (pages.shape[-2] * pb, pb, 1),
+          f"pages: uint8 [{'layers, ' if layered else ''}n_pages, heads, {pb}] for head dim {hd}, a layer's pages contiguous; got {tuple(pages.shape)} {pages.dtype}")
+    layers, stride = (pages.shape[0], pages.stride(0)) if pages.dim() == 4 else (1, 0)
+    _need(layers == 1 or stride >= pages.shape[-3] * pages.shape[-2] * pb, "pages: layers overlap")
+    return layers, stride, pages.shape[-3], pages.shape[-2]
+
+
+def _kv4_rows(t, hd):
+    """a [tokens, heads, hd] bf16 view whose 8-element pieces are 16-byte aligned (copied only if it is not one)"""
+    _need(t.dtype == bf16 and t.dim() == 3 and t.shape[2] == hd, f"expected bf16 [tokens, heads, {hd}], got {t.dtype} {tuple(t.shape)}")
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def kv4_write(k, v, pages, slots):
+    """quantise k and v [tokens, heads, hd] (bf16 views, e.g. a prefill's rotated keys) into the slots [tokens] (int64; slot s = token s % 32 of page s // 32; a slot
+    outside the pool: the token is not written) of one layer's pages [n_pages, heads, kv4_page_bytes(hd)]."""
+    hd = k.shape[-1]
+    _, _, n_pages, heads = _kv4_pool(pages, hd)
+    _need(k.shape == v.shape and k.shape[1] == heads, f"k {tuple(k.shape)}, v {tuple(v.shape)}: [tokens, {heads}, {hd}]")
+    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.numel() == k.shape[0] and slots.is_contiguous(), "slots: contiguous int64 [tokens]")
+    _same_device(pages, k, v, slots)
+    k, v = _kv4_rows(k, hd), _kv4_rows(v, hd)
+    check(_lib.lib().unimp_kv4_write(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), pages.data_ptr(), n_pages, heads, hd,
+                                      slots.data_ptr(), k.shape[0], _stream()), "kv4_write")
+
+
+def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows, pages, slots):
+    """decode step on the 4-bit cache: rotate q and k of every row (row r with ITS table row cos_rows / sin_rows [rows, rot // 2]; rot = 0: none), quantise the
+    rotated k and v into slot slots[r] of one layer's pages, return the rotated q [rows, heads, hd].  Operand layout of decode_rope_append; qkv2d is left unrotated."""
+    _, _, n_pages, ph = _kv4_pool(pages, hd)
+    rows = qkv2d.shape[0]
+    _need(qkv2d.dtype == bf16 and qkv2d.dim() == 2 and qkv2d.stride(1) == 1 and ph == heads, f"qkv: bf16 rows with unit stride, {ph} heads")
+    _need(len(offs) == 3 and min(offs) >= 0 and head_stride >= 0 and max(offs) + (heads - 1) * head_stride + hd <= qkv2d.shape[1], "q / k / v offsets outside the row")
+    _need(0 <= rot <= hd and rot % 2 == 0, f"rot {rot}: even, at most the head dim")
+    _need(slots.dtype == torch.int64 and slots.shape == (rows,) and slots.is_contiguous(), "slots: contiguous int64 [rows]")
+    if rot:
+        _need(all(t.dtype == torch.float32 and t.shape == (rows, rot // 2) and t.is_contiguous() for t in (cos_rows, sin_rows)), "cos / sin: contiguous fp32 [rows, rot // 2]")
+    _same_device(pages, qkv2d, slots, cos_rows if rot else None, sin_rows if rot else None)
+    q = torch.empty((rows, heads, hd), dtype=bf16, device=qkv2d.device)
+    check(_lib.lib().unimp_kv4_rope_append(qkv2d.data_ptr(), qkv2d.stride(0), head_stride, rows, heads, hd, offs[0], offs[1], offs[2], rot, _p(cos_rows) if rot else 0,
+                                            _p(sin_rows) if rot else 0, q.data_ptr(), pages.data_ptr(), n_pages, slots.data_ptr(), _stream()), "kv4_rope_append")
+    return q
+
+
+def kv4_read(pages, slots, hd):
+    """the values held in slots [tokens] (int64; outside the pool: zeros) of pages [(layers,) n_pages, heads, kv4_page_bytes(hd)] -> k, v bf16
+    [(layers,) tokens, heads, hd]: exactly what the attention multiplies"""
+    layers, stride, n_pages, heads = _kv4_pool(pages, hd, layered=True)
+    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.is_contiguous(), "slots: contiguous int64 [tokens]")
+    _same_device(pages, slots)
+    shape = tuple(pages.shape[:-3]) + (slots.numel(), heads, hd)
+    k, v = torch.empty(shape, dtype=bf16, device=pages.device), torch.empty(shape, dtype=bf16, device=pages.device)
+    check(_lib.lib().unimp_kv4_read(pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), slots.numel(), k.data_ptr(), v.data_ptr(), _stream()), "kv4_read")
+    return k, v
+
+
+def page_tables_extend(tables, mapped, cached, new, free_pages, cursor, max_tokens, cover=None, group=1, shared_len=None):
+    """page tables and slots on the GPU from the rows' lengths, one launch.  tables int32 [rows, width] (in place: new columns are filled in), mapped int32 [rows] columns
+    filled in so far, cached / new int32 [rows] tokens in the cache and arriving, cover int32 [rows] tokens that the pages have to reach (None: cached + new),
+    free_pages int32 [n] handed out from cursor (int32 [1]) on, max_tokens: room for the slots (at least the sum of new).  group > 1 with shared_len (int32
+    [rows // group]): the rows of a group take their first row's pages below shared_len // 32 columns.
+    Returns (mapped, cursor, slots, cu): the new column counts and free-list position (above n: pages were missing, their columns are -1), slots int64 [max_tokens] of
+    the new tokens in packed order (-1: none) and int32 [rows + 1] the packed index of every row's first new token."""
+    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous() and tables.numel() > 0, "tables: contiguous int32 [rows, width]")
+    rows, width = tables.shape
+    for name, t, n in (("mapped", mapped, rows), ("cached", cached, rows), ("new", new, rows), ("cover", cover, rows), ("cursor", cursor, 1),
+                       ("shared_len", shared_len, rows // max(group, 1))):
+        _need(t is None or (t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()), f"{name}: contiguous int32 [{n}]")
+    _need(free_pages.dtype == torch.int32 and free_pages.dim() == 1 and free_pages.is_contiguous() and free_pages.numel() < 2 ** 31, "free_pages: contiguous int32 [n]")
+    _need(group >= 1 and rows % group == 0 and max_tokens >= 0, f"{rows} rows in groups of {group}, room for {max_tokens} tokens")
+    _same_device(tables, mapped, cached, new, free_pages, cursor, cover, shared_len)
+    i32 = lambda n: torch.empty(n, dtype=torch.int32, device=tables.device)
+    mapped_out, cursor_out, cu, slots = i32(rows), i32(1), i32(rows + 1), torch.empty(max_tokens, dtype=torch.int64, device=tables.device)
+    check(_lib.lib().unimp_page_tables_extend(tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), _p(cover), free_pages.data_ptr(),
+                                               free_pages.numel(), cursor.data_ptr(), group, _p(shared_len), mapped_out.data_ptr(), cursor_out.data_ptr(),
+                                               slots.data_ptr(), max_tokens, cu.data_ptr(), _stream()), "page_tables_extend")
+    return mapped_out, cursor_out, slots, cu
+
+
+def kv4_reorder_beams(pages, tables, group, src_local, pos):
+    """beam search on the 4-bit cache, in place, all layers in one launch: row j of every group goes on with the hypothesis of row src_local[g * group + j] (int64, index
+    inside the group); pos int64 [rows] = tokens cached (the same in a group).  Full pages change hands in tables [rows, width] (int32), the page that is being
+    filled is copied in pages [(layers,) n_pages, heads, page bytes] into the row's own."""
+    hd = _kv4_hd(pages)
+    layers, stride, n_pages, heads = _kv4_pool(pages, hd, layered=True)
+    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous() and group >= 1 and tables.shape[0] % group == 0, "tables: contiguous int32 [rows, width]")
+    _need(all(t.dtype == torch.int64 and t.shape == (tables.shape[0],) and t.is_contiguous() for t in (src_local, pos)), "src_local, pos: contiguous int64 [rows]")
+    _same_device(pages, tables, src_local, pos)
+    check(_lib.lib().unimp_kv4_reorder_beams(pages.data_ptr(), stride, layers, n_pages, heads, hd, tables.data_ptr(), tables.shape[1], group, tables.shape[0] // group,
+                                              src_local.data_ptr(), pos.data_ptr(), _stream()), "kv4_reorder_beams")
+
+
+def _kv4_hd(pages):
+    for hd in (64, 80, 128):
+        if pages.shape[-1] == kv4_page_bytes(hd):
+            return hd
+    raise ValueError(f"pages of {pages.shape[-1]} bytes: {[kv4_page_bytes(h) for h in (64, 80, 128)]} are those of head dims 64, 80 and 128")
+
+
+def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_len=None, out=None):
+    """attention of one new token per row over the 4-bit cache: q [rows, heads, hd] (bf16 view) against the first lens[r] (int32 [rows]) tokens of the pages that
+    tables [rows, width] (int32) name in one layer's pool [n_pages, kv heads, page bytes]; heads a multiple of kv heads.  alibi: fp32 [heads] slopes.  A row of length 0
+    gives zeros; a page id outside the pool hides its tokens.  group > 1 with shared_len (int32 [rows // group]): the rows of a group (the beams of a prompt) name the
+    same pages below shared_len // 32 columns; those are read once per group.  Returns o [rows, heads, hd]."""
+    _need(q.dim() == 3 and q.dtype == bf16 and q.stride(2) == 1, "q: bf16 [rows, heads, hd] with unit dim stride")
+    rows, heads, hd = q.shape
+    _, _, n_pages, kv_heads = _kv4_pool(pages, hd)
+    _need(kv_heads > 0 and heads % kv_heads == 0 and heads // kv_heads <= 16, f"{heads} query heads on {kv_heads} key heads: a multiple, at most 16 to one")
+    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == rows and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [rows, width], unit column stride")
+    _need(lens.dtype == torch.int32 and lens.shape == (rows,) and lens.is_contiguous(), "lens: contiguous int32 [rows]")
+    if alibi is not None:
+        _need(alibi.dtype == torch.float32 and alibi.numel() == heads and alibi.is_contiguous(), "alibi: contiguous fp32 [heads]")
+    if shared_len is not None:
+        _need(group >= 1 and rows % group == 0 and shared_len.dtype == torch.int32 and shared_len.numel() == rows // group and shared_len.is_contiguous(),
+              "shared_len: contiguous int32 [rows // group]")
+    if out is None:
+        out = torch.empty((rows, heads, hd), dtype=bf16, device=q.device)
+    _need(out.dtype == bf16 and out.shape == q.shape and out.stride(2) == 1, "out: bf16 like q, unit dim stride")
+    _same_device(pages, q, tables, lens, alibi, shared_len, out)
+    d = _lib.Kv4AttnDesc()
+    d.q, d.q_row_stride, d.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    d.pages, d.n_pages, d.kv_heads, d.hd = pages.data_ptr(), n_pages, kv_heads, hd
+    d.tables, d.table_stride, d.width, d.lens = tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr()
+    d.rows, d.heads, d.scale, d.alibi_slopes = rows, heads, scale, _p(alibi)
+    d.out, d.o_row_stride, d.o_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
+    d.group, d.shared_len = (group, shared_len.data_ptr()) if group > 1 and shared_len is not None else (1, None)
+    L = _lib.lib()
+    n = L.unimp_kv4_attn_workspace(C.byref(d))
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None          # of this call: nothing that two streams or graphs could share
+    check(L.unimp_kv4_attn_decode(C.byref(d), _p(ws), _stream()), "kv4_attn_decode")
+    return out
