@@ -1,97 +1,381 @@
-// Attention of one new token per row over the 4-bit pages (kv4.h): o = softmax(scale q k_j + slope j) v_j over the row's cached tokens j < len.
-// (eval_rec.py:100-110 / eval_exp.py:103-113 / eval_img_gen.py:102-111: the cached decode step inside Flamingo.generate.)
+// Attention of one new token per row over the 4-bit pages (kv4.h): o = softmax_j(scale q k_j + slope j) v_j over the row's cached tokens j < len
+// (eval_rec.py:100-110 / eval_exp.py:103-113 / eval_img_gen.py:102-111: the cached decode step inside Flamingo.generate).
+//
+// One wave takes one page (32 tokens) at a time, everything on the matrix pipe, K and V never unpacked in LDS:
+//   scores   S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4: A = the page's K codes and scale bytes AS STORED (kv4.h: a lane's operand is one 16-byte load),
+//            B = the queries in its 16 columns, each 32-dim block of a query as e4m3 hi + lo under a shared power-of-two scale.  A bf16 has 8 significant bits, e4m3 four:
+//            hi + lo is exact for elements down to 2^-10 of the block's largest and within 2^-17 of that one below.
+//   softmax  online, base 2, lane (column c, group g) holds tokens 16 h + 4 g + e of the page; the running maximum moves only when a score exceeds it by 2^10 (p <= 1024
+//            costs nothing in fp32), so the common page has no cross-lane step and no rescale.
+//   o^T     += V^T P^T on v_mfma_f32_16x16x32_bf16: A = V's nibbles through v_cvt_scalef32_pk_bf16_fp4 (exact), B = p times the token's V scale, which differs per 32 dims.
+//            p is split in two bf16 (16 bits kept).  The scale blocks and the two halves are COLUMNS of B where the queries leave room: with one or two queries
+//            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
+//            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 2: 16 queries, block and half as products.
+// Bound by the bytes of the pages: 17 / 32 of a byte per element.
 #include "kv4.h"
 #include "unimp_hip.h"
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
   int rows, heads; float scale; const float* alibi; bf16* o; long o_rs, o_hs; int group; const int32_t* shared;
+  int chunk, slots;                    // pages of a workgroup; partial slots per row and part (prefix / rest)
+  float* ws;                           // null: a workgroup holds a row's whole range and writes o
 };
 
-// one block per (row, query head), a wave takes every fourth tile of 64 tokens: lane = token for the scores, lane = dim for the values
-template <int D>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
+template <int D, int MODE> struct Kv4Cols {
+  static constexpr int NBP = D == 64 ? 2 : 4;                                     // scale blocks as columns (three of head dim 80 in four)
+  static constexpr int VAR = MODE == 0 ? 2 * NBP : MODE == 1 ? NBP : 1, Q = 16 / VAR;
+};
+
+template <int D> struct Kv4Frag {        // one page as a wave holds it
+  u32x4 k[2]; u32x4 v0; u32x4 v1; uint32_t ks; u32x2 vs;
+};
+
+template <int D, int MODE, int NW, bool ALIBI>
+__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   using P = Kv4<D>;
-  __shared__ float qs[D], ps[4][64], part[4][D], pm[4], pl[4];
-  __shared__ int pgs[4][2];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.y, h = blockIdx.x, kvh = h / (a.heads / a.kv_heads);
-  const int len = min(max(a.lens[row], 0), a.width * KV4_PAGE);
-  for (int d = tid; d < D; d += 256) qs[d] = bf2f(a.q[row * a.q_rs + h * a.q_hs + d]) * a.scale * 1.4426950408889634f;
-  __syncthreads();
-  const float slope = a.alibi ? a.alibi[h] * 1.4426950408889634f : 0.f;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int base = w * 64; base < len; base += 256) {
-    const int t = base + lane;
-    int pg = t < len ? a.tables[row * a.t_stride + (t >> 5)] : -1;
-    if (pg >= a.n_pages) pg = -1;
-    if (!(lane & 31)) pgs[w][lane >> 5] = pg;
-    float s = -INFINITY;
-    if (pg >= 0) {
-      const uint8_t* page = a.pages + ((long)pg * a.kv_heads + kvh) * P::BYTES;
-      s = 0.f;
-      for (int b = 0; b < P::NB; ++b) {
-        const int nd = b == P::NB - 1 ? P::BLK_LAST : 32;
-        float x = 0.f;
-        for (int j = 0; j < nd; j += 8) {
-          const uint32_t c = *(const uint32_t*)(page + P::k_byte(t & 31, b) + j / 2);
-          for (int i = 0; i < 8; ++i) x = fmaf(kv4_value((c >> (4 * i)) & 15u), qs[32 * b + j + i], x);
-        }
-        s = fmaf(x, kv4_scale(page[P::ks_byte(t & 31, b)]), s);
+  using CO = Kv4Cols<D, MODE>;
+  constexpr int NI = P::NI;
+  __shared__ float so[NW][CO::Q][D], sm[NW][CO::Q], sl[NW][CO::Q];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, G = a.heads / a.kv_heads;
+  // ---- which rows and columns of their tables: z < rows: the row's own pages; above: the pages that a group shares, for all its queries at once
+  const bool prefix = (int)blockIdx.z >= a.rows;
+  const int row = prefix ? ((int)blockIdx.z - a.rows) * a.group : (int)blockIdx.z;
+  const int nq = prefix ? a.group * G : G;
+  const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
+  const int qi = col / CO::VAR, var = col % CO::VAR;
+  const int my_row = prefix ? row + min(qi / G, a.group - 1) : row, my_head = kvh * G + (qi < nq ? qi % G : 0);
+  const int my_len = min(max(a.lens[my_row], 0), a.width * KV4_PAGE);
+  int top = my_len;                                                               // the longest of the rows here
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 16));
+  top = __builtin_amdgcn_readfirstlane(top);
+  const int cols = (top + KV4_PAGE - 1) / KV4_PAGE;
+  const int first = prefix ? 0 : min(shared, cols), last = prefix ? min(shared, cols) : cols;
+  const int c0 = first + blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, last);
+  if (c0 >= c1 && !(a.ws == nullptr)) return;                                     // nothing here (a row without tokens still gets its zeros)
+
+  // ---- page ids of this wave: page c0 + w + NW k in lane k
+  const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;
+  int ids = -1;
+  if (lane < n) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
+  if (ids >= a.n_pages) ids = -1;
+
+  auto load = [&](Kv4Frag<D>& f, int k) {
+    const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
+    const uint8_t* page = a.pages + ((long)id * a.kv_heads + kvh) * P::BYTES;
+    const u32x4 z = {0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f.k[h] = z;
+      if (D == 128 || g < P::NB - (P::BLK_LAST < 32)) f.k[h] = *(const u32x4*)(page + 512 * g + (16 * h + col) * 16);
+      else if (P::BLK_LAST < 32 && g == P::NB - 1) { const u32x2 t = *(const u32x2*)(page + 512 * g + (16 * h + col) * 8); f.k[h] = u32x4{t[0], t[1], 0, 0}; }
+    }
+    f.ks = 0x7f7f;
+    if (D == 128 || g < P::NB) f.ks = *(const uint16_t*)(page + P::KS + 32 * g + 2 * col);
+    const uint8_t* vp = page + P::VOFF + 4 * (g * D + col * NI);
+    if constexpr (D == 80) {
+      typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4u;
+      f.v0 = *(const u32x4u*)vp; f.v1[0] = *(const uint32_t*)(vp + 16);
+    } else {
+      f.v0 = *(const u32x4*)vp;
+      if (D == 128) f.v1 = *(const u32x4*)(vp + 16);
+    }
+    if constexpr (MODE < 2) {
+      const int b = min(MODE == 0 ? var >> 1 : var, P::NB - 1);
+      f.vs = *(const u32x2*)(page + P::VS + 8 * P::NB * g + 8 * b);
+    }
+  };
+
+  Kv4Frag<D> fa, fb;
+  if (n > 0) load(fa, 0);
+  if (n > 1) load(fb, 1);
+
+  // ---- queries: lane (c, g) holds dims 16 g ... and 64 + 16 g ... of column c's query
+  i32x8 qh, ql;
+  int sb;
+  {
+    const bf16* qp = a.q + (long)my_row * a.q_rs + (long)my_head * a.q_hs;
+    int sx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d0 = 64 * h + 16 * g;
+      float x[16];
+      uint32_t mx = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        x[j] = qi < nq && d0 + j < D ? bf2f(qp[d0 + j]) : 0.f;
+        mx = max(mx, __float_as_uint(x[j]) & 0x7fffffffu);
       }
-      s = fmaf(slope, (float)(t - len + 1), s);
+      mx = max(mx, __shfl_xor(mx, 16, 64));                                       // the other half of the 32-dim block
+      const int eb = (int)(mx >> 23), s = max(eb - 7, 1);
+      sx[h] = eb == 255 ? 127 : s;
+      const float inv = __uint_as_float((uint32_t)(254 - s) << 23);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        int hi = 0, lo = 0;
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[j] * inv, x[j + 1] * inv, hi, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[j + 2] * inv, x[j + 3] * inv, hi, true);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[j] * inv - __builtin_amdgcn_cvt_f32_fp8(hi, 0), x[j + 1] * inv - __builtin_amdgcn_cvt_f32_fp8(hi, 1), lo, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[j + 2] * inv - __builtin_amdgcn_cvt_f32_fp8(hi, 2), x[j + 3] * inv - __builtin_amdgcn_cvt_f32_fp8(hi, 3), lo, true);
+        qh[4 * h + j / 4] = eb == 255 ? 0x7f7f7f7f : hi;                          // an infinite or NaN query: its scores are NaN
+        ql[4 * h + j / 4] = eb == 255 ? 0 : lo;
+      }
     }
-    const float mx = fmaxf(m, wave_max(s)), r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-    const float p = pg < 0 ? 0.f : __builtin_amdgcn_exp2f(s - (mx == -INFINITY ? 0.f : mx));
-    m = mx;
-    l = fmaf(l, r, wave_sum(p));
-    ps[w][lane] = p;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    o0 *= r; o1 *= r;
-    for (int j = 0; j < 64; ++j) {
-      const int pj = pgs[w][j >> 5];
-      if (pj < 0 || base + j >= len) continue;
-      const uint8_t* page = a.pages + ((long)pj * a.kv_heads + kvh) * P::BYTES;
-      const int tt = j & 31, sh = 4 * kv4_nibble(tt);
-      const float pp = ps[w][j];
-      o0 = fmaf(pp, kv4_value((*(const uint32_t*)(page + P::v_dword(tt, lane)) >> sh) & 15u) * kv4_scale(page[P::vs_byte(tt, lane >> 5)]), o0);
-      if (lane + 64 < D) o1 = fmaf(pp, kv4_value((*(const uint32_t*)(page + P::v_dword(tt, lane + 64)) >> sh) & 15u) * kv4_scale(page[P::vs_byte(tt, (lane + 64) >> 5)]), o1);
-    }
-    __builtin_amdgcn_wave_barrier();
+    // the scale operand's lane (c, t) carries block t: blocks 0, 1 are the first halves of groups 0, 2; blocks 2, 3 their second halves
+    const int s0 = __shfl(sx[0], (g & 1) * 32 + col, 64), s1 = __shfl(sx[1], (g & 1) * 32 + col, 64);
+    sb = g < 2 ? s0 : s1;
   }
-  part[w][lane] = o0;
-  if (lane + 64 < D) part[w][lane + 64] = o1;
-  if (!lane) { pm[w] = m; pl[w] = l; }
-  __syncthreads();
-  const float M = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
-  for (int d = tid; d < D; d += 256) {
-    float L = 0.f, x = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const float e = pm[i] == -INFINITY && pl[i] == 0.f ? 0.f : __builtin_amdgcn_exp2f(pm[i] - (M == -INFINITY ? 0.f : M));
-      L = fmaf(pl[i], e, L); x = fmaf(part[i][d], e, x);
+  const float sc = a.scale * 1.4426950408889634f, slope = ALIBI ? a.alibi[my_head] * 1.4426950408889634f : 0.f;
+
+  f32x4 acc[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, mu = 0.f, l = 0.f;                                         // running maximum; the same, 0 while there is none; sum of this lane's tokens
+
+  auto compute = [&](const Kv4Frag<D>& f, int k) {
+    const int c = c0 + w + NW * k;
+    const int vis = __builtin_amdgcn_readlane(ids, k) < 0 ? 0 : my_len - c * KV4_PAGE;      // tokens of this page that the lane's query sees
+    f32x4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const i32x8 ka = {(int)f.k[h][0], (int)f.k[h][1], (int)f.k[h][2], (int)f.k[h][3], 0, 0, 0, 0};
+      const int ks = h ? (int)(f.ks >> 8) : (int)f.ks;
+      f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, qh, z, 4, 0, 0, ks, 0, sb);
+      s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, ql, z, 4, 0, 0, ks, 0, sb);
     }
-    a.o[row * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : x / L);
+    uint32_t vs0, vs1;
+    if constexpr (MODE < 2) { vs0 = f.vs[0]; vs1 = f.vs[1]; }
+    float x[8];
+    const float at = ALIBI ? (float)(c * KV4_PAGE + 4 * g - my_len + 1) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = s[j >> 2][j & 3] * sc;
+      if (ALIBI) x[j] = fmaf(slope, at + (float)(16 * (j >> 2) + (j & 3)), x[j]);
+    }
+    const bool part = __any(vis < KV4_PAGE);
+    if (part) {                                                                   // the last page, or a hidden one
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (16 * (j >> 2) + 4 * g + (j & 3) >= vis) x[j] = -INFINITY;
+    }
+    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(mx > m + 10.f)) {
+      float t = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      t = fmaxf(t, m);
+      const float r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - t);
+      m = t; mu = t == -INFINITY ? 0.f : t;
+      l *= r;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] *= r;
+    }
+    float hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = __builtin_amdgcn_exp2f(x[j] - mu);
+      l += p;
+      hi[j] = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
+      lo[j] = p - hi[j];
+    }
+    auto pack = [](float a0, float a1) { return __builtin_amdgcn_perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u); };      // upper halves
+    auto vscale = [&](uint32_t d, int j) { return __uint_as_float(((d >> (8 * j)) & 0xffu) << 23); };      // byte 255 (not a number): infinity, 0 x infinity = NaN
+    auto value = [&](int i) {                                                     // operand of dims 16 i + col
+      const uint32_t d = i < 4 ? f.v0[i & 3] : f.v1[i & 3];
+      union { bf16x2 h[4]; bf16x8 v; } u;
+      u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 0);
+      u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 1);
+      u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 2);
+      u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 3);
+      return u.v;
+    };
+    union B { uint32_t d[4]; bf16x8 v; };
+    auto hide = [&](uint32_t& d0, uint32_t& d1) {                                 // scale bytes of tokens that are not there: 0, whatever memory holds
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (4 * g + j >= vis) d0 &= ~(0xffu << (8 * j));
+          if (16 + 4 * g + j >= vis) d1 &= ~(0xffu << (8 * j));
+        }
+      }
+    };
+    if constexpr (MODE == 0) {
+      hide(vs0, vs1);
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = ((var & 1) ? lo[j] : hi[j]) * vscale(j < 4 ? vs0 : vs1, j & 3);
+      B b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b.d[j] = pack(y[2 * j], y[2 * j + 1]);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i] = MFMA16(value(i), b.v, acc[i]);
+    } else if constexpr (MODE == 1) {
+      hide(vs0, vs1);
+      B bh, bl;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s0 = vscale(j < 2 ? vs0 : vs1, 2 * j & 3), s1 = vscale(j < 2 ? vs0 : vs1, (2 * j + 1) & 3);
+        bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);
+        bl.d[j] = pack(lo[2 * j] * s0, lo[2 * j + 1] * s1);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
+    } else {
+      const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
+      const uint8_t* sp = a.pages + ((long)id * a.kv_heads + kvh) * P::BYTES + P::VS + 8 * P::NB * g;
+#pragma unroll
+      for (int blk = 0; blk < P::NB; ++blk) {
+        const u32x2 d = *(const u32x2*)(sp + 8 * blk);
+        uint32_t d0 = d[0], d1 = d[1];
+        hide(d0, d1);
+        B bh, bl;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float s0 = vscale(j < 2 ? d0 : d1, 2 * j & 3), s1 = vscale(j < 2 ? d0 : d1, (2 * j + 1) & 3);
+          bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);
+          bl.d[j] = pack(lo[2 * j] * s0, lo[2 * j + 1] * s1);
+        }
+#pragma unroll
+        for (int i = 2 * blk; i < 2 * blk + 2; ++i) if (i < NI) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
+      }
+    }
+  };
+
+  for (int k = 0; k < n; k += 2) {
+    compute(fa, k);
+    if (k + 2 < n) load(fa, k + 2);
+    if (k + 1 < n) {
+      compute(fb, k + 1);
+      if (k + 3 < n) load(fb, k + 3);
+    }
+  }
+
+  // ---- join the waves: lane (c, g) holds dims 16 i + 4 g + e of column c
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    f32x4 x = acc[i];
+    if constexpr (MODE == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], 1, 64);                // the two halves of p
+    }
+    const bool mine = MODE == 0 ? var == 2 * (i >> 1) : MODE == 1 ? var == (i >> 1) : true;
+    if (mine && qi < nq) *(f32x4*)&so[w][qi][16 * i + 4 * g] = x;
+  }
+  if (var == 0 && g == 0) { sm[w][qi] = m; sl[w][qi] = l; }
+  __syncthreads();
+  for (int x = tid; x < nq * D; x += 64 * NW) {
+    const int qq = x / D, d = x - qq * D;
+    float M = sm[0][qq];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) M = fmaxf(M, sm[i][qq]);
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const float e = sm[i][qq] == -INFINITY && sl[i][qq] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sm[i][qq] - (M == -INFINITY ? 0.f : M));
+      L = fmaf(sl[i][qq], e, L); o = fmaf(so[i][qq][d], e, o);
+    }
+    const int r = prefix ? row + qq / G : row, h = kvh * G + qq % G;
+    if (a.ws) {
+      const int parts = a.group > 1 ? 2 : 1;                                      // prefix slots, then the row's own
+      float* p = a.ws + (((long)r * a.heads + h) * parts * a.slots + (prefix ? 0 : (parts - 1) * a.slots) + blockIdx.x) * (D + 2);
+      p[d] = o;
+      if (d == 0) { p[D] = M; p[D + 1] = L; }
+    } else {
+      a.o[r * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : o / L);
+    }
   }
 }
 
-extern "C" int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc*) { return 0; }
+// the partials of a (row, head), in slot order
+template <int D>
+__global__ __launch_bounds__(D) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
+  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
+  const int len = min(max(a.lens[row], 0), a.width * KV4_PAGE), cols = (len + KV4_PAGE - 1) / KV4_PAGE;
+  const int parts = a.group > 1 ? 2 : 1;
+  int np = 0;
+  if (a.group > 1) {
+    int top = 0;                                                                  // a group's prefix workgroups go as far as its longest row
+    for (int j = 0; j < a.group; ++j) top = max(top, min(max(a.lens[row / a.group * a.group + j], 0), a.width * KV4_PAGE));
+    np = min(min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width), (top + KV4_PAGE - 1) / KV4_PAGE);
+  }
+  const int own = max(cols - (a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0), 0);
+  const float* base = a.ws + ((long)row * a.heads + h) * parts * a.slots * (D + 2);
+  const int n0 = (np + a.chunk - 1) / a.chunk, n1 = (own + a.chunk - 1) / a.chunk;
+  float M = -INFINITY;
+  for (int i = 0; i < n0 + n1; ++i) M = fmaxf(M, base[(long)(i < n0 ? i : (parts - 1) * a.slots + i - n0) * (D + 2) + D]);
+  float L = 0.f, o = 0.f;
+  for (int i = 0; i < n0 + n1; ++i) {
+    const float* p = base + (long)(i < n0 ? i : (parts - 1) * a.slots + i - n0) * (D + 2);
+    const float pm = p[D], pl = p[D + 1], e = pm == -INFINITY && pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(pm - (M == -INFINITY ? 0.f : M));
+    L = fmaf(pl, e, L); o = fmaf(p[d], e, o);
+  }
+  a.o[row * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : o / L);
+}
 
-extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* workspace, void* stream) {
-  (void)workspace;
+struct Kv4Plan { int mode, nw, chunk, slots, group; int64_t floats; };
+static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
+  Kv4Plan p;
+  const int G = d->heads / d->kv_heads, nbp = d->hd == 64 ? 2 : 4;
+  p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 ? d->group : 1;
+  const int nq = p.group > 1 ? p.group * G : G;                                   // one launch serves both kinds of workgroups
+  p.mode = nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : 2;
+  const long units = (long)d->rows * d->kv_heads;
+  p.nw = p.mode < 2 && units < 512 ? 8 : 4;
+  const long want = (long)d->width * units / 2048;                                // pages of a workgroup that leave 2048 workgroups
+  p.chunk = (int)(want < 4 * p.nw ? 4 * p.nw : want > 32 * p.nw ? 32 * p.nw : want);
+  p.slots = d->width > 0 ? (d->width + p.chunk - 1) / p.chunk : 1;
+  p.floats = p.group == 1 && p.slots == 1 ? 0 : (int64_t)units * G * (p.group > 1 ? 2 : 1) * p.slots * (d->hd + 2);
+  return p;
+}
+static int kv4_attn_check(const unimp_kv4_attn_desc* d) {
   if (!d || !d->q || !d->pages || !d->tables || !d->lens || !d->out) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: null pointer");
-  if (d->rows <= 0 || d->heads <= 0) return UNIMP_OK;
-  if (d->kv_heads <= 0 || d->heads % d->kv_heads || d->heads / d->kv_heads > 16 || d->width < 0 || d->width > (1 << 26) || d->rows > 65535 || d->heads > 65535)
-    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 65535 rows, 2^26 pages of a row");
+  if (d->kv_heads <= 0 || d->heads < 0 || d->heads % d->kv_heads || d->heads / d->kv_heads > 16 || d->width < 0 || d->width > (1 << 26) || d->rows < 0 || d->rows > 32767 ||
+      d->heads > 65535 || d->n_pages <= 0)
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 32767 rows, 2^26 pages of a row; a pool with pages");
   if (d->hd != 64 && d->hd != 80 && d->hd != 128) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
   if ((uintptr_t)d->pages & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_attn_decode: 16-byte aligned pages");
+  return UNIMP_OK;
+}
+
+extern "C" int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc* d) { return kv4_attn_check(d) || !d->rows || !d->heads ? 0 : kv4_plan(d).floats; }
+
+template <int D>
+static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
+  const dim3 grid(p.slots, a.kv_heads, a.rows + (p.group > 1 ? a.rows / p.group : 0));
+#define KV4_L(M, W)                                                                                          \
+  do {                                                                                                       \
+    if (a.alibi) hipLaunchKernelGGL((kv4_attn_kernel<D, M, W, true>), grid, dim3(64 * W), 0, s, a);          \
+    else hipLaunchKernelGGL((kv4_attn_kernel<D, M, W, false>), grid, dim3(64 * W), 0, s, a);                 \
+  } while (0)
+  if (p.mode == 0 && p.nw == 8) KV4_L(0, 8);
+  else if (p.mode == 0) KV4_L(0, 4);
+  else if (p.mode == 1 && p.nw == 8) KV4_L(1, 8);
+  else if (p.mode == 1) KV4_L(1, 4);
+  else KV4_L(2, 4);
+#undef KV4_L
+  if (a.ws) hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(D), 0, s, a);
+}
+
+extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* workspace, void* stream) {
+  const int rc = kv4_attn_check(d);
+  if (rc) return rc;
+  if (!d->rows || !d->heads) return UNIMP_OK;
+  const Kv4Plan p = kv4_plan(d);
+  if (p.floats && !workspace) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: workspace of unimp_kv4_attn_workspace floats");
   Kv4AttnArgs a{(const bf16*)d->q, d->q_row_stride, d->q_head_stride, (const uint8_t*)d->pages, d->n_pages, d->kv_heads, d->tables, d->table_stride, d->width, d->lens,
-                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, d->group, d->shared_len};
-  dim3 grid(d->heads, d->rows);
+                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, p.group, d->shared_len, p.chunk, p.slots,
+                p.floats ? workspace : nullptr};
   switch (d->hd) {
-    case 64: hipLaunchKernelGGL((kv4_attn_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, a); break;
-    case 80: hipLaunchKernelGGL((kv4_attn_kernel<80>), grid, dim3(256), 0, (hipStream_t)stream, a); break;
-    case 128: hipLaunchKernelGGL((kv4_attn_kernel<128>), grid, dim3(256), 0, (hipStream_t)stream, a); break;
-    default: return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
+    case 64: kv4_attn_launch<64>(a, p, (hipStream_t)stream); break;
+    case 80: kv4_attn_launch<80>(a, p, (hipStream_t)stream); break;
+    default: kv4_attn_launch<128>(a, p, (hipStream_t)stream);
   }
   return unimp_check_launch("kv4_attn_decode");
 }
