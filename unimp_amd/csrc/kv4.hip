@@ -18,85 +18,146 @@ template <typename F> static int kv4_for_hd(int hd, F f) {
 }
 extern "C" int unimp_kv4_page_bytes(int hd) { return hd == 64 || hd == 80 || hd == 128 ? 32 * hd + 64 * ((hd + 31) / 32) : -1; }
 
+// ------------------------------------------------------------------------------------------- runs of slots
+// A RUN is a maximal stretch of consecutive rows whose slots are consecutive inside one page; a workgroup (chunk of 32 rows, some heads) owns the runs that START
+// in its chunk (a run has at most 32 rows: it looks 31 rows ahead), so every row is moved once and every page is touched by one wave per run, whatever the
+// alignment of the rows to the pages.  sl[1 + i] = slot of row i0 + i, -1: none.
+__device__ __forceinline__ void kv4_load_slots(int64_t (&sl)[65], const int64_t* __restrict__ slots, long i0, long tokens, long n_pages) {
+  if (threadIdx.x < 65) {
+    const long i = i0 - 1 + (int)threadIdx.x;
+    const int64_t s = i >= 0 && i < tokens ? slots[i] : -1;
+    sl[threadIdx.x] = s >= 0 && s < n_pages * KV4_PAGE ? s : -1;
+  }
+  __syncthreads();
+}
+// rows of the run that starts at row a (0: none starts there)
+__device__ __forceinline__ int kv4_run(const int64_t (&sl)[65], int a) {
+  const int64_t s0 = sl[a + 1];
+  if (s0 < 0 || !(sl[a] < 0 || sl[a] + 1 != s0 || (s0 & 31) == 0)) return 0;
+  const int lane = lane_id(), t0 = (int)(s0 & 31);
+  const bool on = lane < 32 && a + lane < 64 && t0 + lane < 32 && sl[min(a + 1 + lane, 64)] == s0 + lane;      // lane 0: itself
+  return __builtin_ctzll(~__ballot(on));
+}
+// eight dwords of eight nibbles, turned round: out[i] nibble j = in[j] nibble i
+__device__ __forceinline__ void kv4_turn8(uint32_t (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = x[i], b = x[i + 4];
+    x[i] = __builtin_amdgcn_perm(b, a, 0x05040100u); x[i + 4] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  }
+#pragma unroll
+  for (int h = 0; h < 8; h += 4)
+#pragma unroll
+    for (int i = h; i < h + 2; ++i) {
+      const uint32_t a = x[i], b = x[i + 2];
+      x[i] = __builtin_amdgcn_perm(b, a, 0x06020400u); x[i + 2] = __builtin_amdgcn_perm(b, a, 0x07030501u);
+    }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint32_t a = x[i], b = x[i + 1], m = 0x0f0f0f0fu;
+    x[i] = (a & m) | ((b << 4) & ~m); x[i + 1] = ((a >> 4) & m) | (b & ~m);
+  }
+}
+__device__ __forceinline__ void wave_lds_fence() {                   // LDS of this wave's other lanes
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // ------------------------------------------------------------------------------------------- write
-// A RUN is a maximal stretch of consecutive rows whose slots are consecutive inside one page; a workgroup (chunk of 32 rows, head) owns the runs that START
-// in its chunk (a run has at most 32 rows: it looks 31 rows ahead), so every row is read once, by one workgroup, whatever the alignment of the rows to the
-// pages.  A V dword holds 8 tokens of one dim: the codes of a run turn round in LDS and a dword whose 8 tokens are all in the run is stored; the dwords at
-// the ragged ends of a run change their nibbles by atomic and + or (another workgroup may hold the other nibbles; the fields are disjoint, the result does not
-// depend on the order).
+// A wave per (run, head).  Four lanes hold an MX block of a token (16-byte loads, the block's maximum by two lane exchanges); V's codes turn round (8 tokens x 8 dims
+// per lane) through LDS; the page is put together in LDS and leaves in 16-byte stores.  A run that does not fill its page writes its own bytes, and its nibbles of V dwords
+// that other runs share by atomic and + or: the fields are disjoint, the result does not depend on the order.
+#define KV4_HEADS 8                                                  // heads of a workgroup
 template <int D>
 __global__ __launch_bounds__(256) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
                                                         uint8_t* __restrict__ pages, long n_pages, int heads, const int64_t* __restrict__ slots, long tokens) {
   using P = Kv4<D>;
+  constexpr int PASSES = 2 * P::NB, X = D / 8;                       // (token, block) pairs in sixteens; 8-dim pieces of a row
   __shared__ int64_t sl[65];
-  __shared__ uint8_t vc[32][D + 4];
-  const int tid = threadIdx.x, head = blockIdx.y;
+  __shared__ __attribute__((aligned(16))) uint8_t image[4][P::BYTES];
+  __shared__ uint32_t turn[4][32 * X];
+  const int lane = lane_id(), w = threadIdx.x >> 6, quad = lane & 3;
   const long i0 = (long)blockIdx.x * 32;
-  if (tid < 65) {
-    const long i = i0 - 1 + tid;
-    const int64_t s = i >= 0 && i < tokens ? slots[i] : -1;
-    sl[tid] = s >= 0 && s < n_pages * KV4_PAGE ? s : -1;
-  }
-  __syncthreads();
-  for (int a = 0; a < 32;) {                                        // rows i0 + a: uniform over the workgroup
+  kv4_load_slots(sl, slots, i0, tokens, n_pages);
+  uint8_t* im = image[w];
+  uint32_t* tv = turn[w];
+  for (int a = 0; a < 32;) {
+    const int n = kv4_run(sl, a);
+    if (!n) { ++a; continue; }                                       // no slot, or the tail of the previous chunk's last run
     const int64_t s0 = sl[a + 1];
-    const bool starts = s0 >= 0 && (sl[a] < 0 || sl[a] + 1 != s0 || (s0 & 31) == 0);
-    if (!starts) { ++a; continue; }                                 // no slot, or the tail of the previous chunk's last run
-    int n = 1;
     const int t0 = (int)(s0 & 31);
-    while (t0 + n < 32 && a + n < 64 && sl[a + 1 + n] == s0 + n) ++n;
-    uint8_t* page = pages + ((s0 >> 5) * heads + head) * (long)P::BYTES;
-    const bool is_v = tid >= 128;
-    const int w = tid & 127, t = w / P::NB, b = w - t * P::NB;      // (token, block): 32 NB <= 128
-    if (t < n) {
-      const bf16* x = (is_v ? v + (i0 + a + t) * v_ts + head * v_hs : k + (i0 + a + t) * k_ts + head * k_hs) + 32 * b;
-      const int nd = b == P::NB - 1 ? P::BLK_LAST : 32;
-      float f[32];
-      uint32_t m = 0;
+    for (int head = blockIdx.y * KV4_HEADS + w; head < min((int)(blockIdx.y + 1) * KV4_HEADS, heads); head += 4) {
+      uint8_t* page = pages + ((s0 >> 5) * heads + head) * (long)P::BYTES;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        bf16x8 u = {};
-        if (8 * c < nd) u = *(const bf16x8*)(x + 8 * c);
+      for (int kind = 0; kind < 2; ++kind) {
+        bf16x8 u[PASSES];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { f[8 * c + j] = bf2f(u[j]); m = max(m, __float_as_uint(f[8 * c + j]) & 0x7fffffffu); }
+        for (int ps = 0; ps < PASSES; ++ps) {                        // all loads of the half page first
+          const int pr = ps * 16 + (lane >> 2), t = pr / P::NB, b = pr - t * P::NB, d = 32 * b + 8 * quad;
+          u[ps] = bf16x8{};
+          if (t >= t0 && t < t0 + n && d < D)
+            u[ps] = *(const bf16x8*)(kind ? v + (i0 + a + t - t0) * v_ts + head * v_hs + d : k + (i0 + a + t - t0) * k_ts + head * k_hs + d);
+        }
+#pragma unroll
+        for (int ps = 0; ps < PASSES; ++ps) {
+          const int pr = ps * 16 + (lane >> 2), t = pr / P::NB, b = pr - t * P::NB, d = 32 * b + 8 * quad;
+          float f[8];
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { f[j] = bf2f(u[ps][j]); m = max(m, __float_as_uint(f[j]) & 0x7fffffffu); }
+          m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));       // lane ^ 1
+          m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));       // lane ^ 2
+          const int sb = kv4_scale_byte((int)(m >> 23));
+          const float scale = __uint_as_float((uint32_t)(sb == 255 ? 127 : sb) << 23);
+          uint32_t r = 0;
+          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[0], f[1], scale, 0);
+          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[2], f[3], scale, 1);
+          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[4], f[5], scale, 2);
+          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[6], f[7], scale, 3);
+          if (sb == 255) r = 0;
+          if (d < D) {
+            if (!kind) *(uint32_t*)(im + P::k_byte(t, b) + 4 * quad) = r;
+            else tv[t * X + (d >> 3)] = r;
+          }
+          if (!quad) im[kind ? P::vs_byte(t, b) : P::ks_byte(t, b)] = (uint8_t)sb;
+        }
       }
-      const int sb = kv4_scale_byte((int)(m >> 23));
-      const float scale = __uint_as_float((uint32_t)(sb == 255 ? 127 : sb) << 23);
-      uint32_t q[4];
+      wave_lds_fence();
+      for (int x = lane; x < 4 * X; x += 64) {                       // lane: 8 tokens of group g, 8 dims
+        const int g = x / X, c8 = x - g * X;
+        uint32_t y[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r = 0;
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c], f[8 * c + 1], scale, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 2], f[8 * c + 3], scale, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 4], f[8 * c + 5], scale, 2);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[8 * c + 6], f[8 * c + 7], scale, 3);
-        q[c] = sb == 255 ? 0u : r;
+        for (int j = 0; j < 8; ++j) y[j] = tv[(16 * (j >> 2) + 4 * g + (j & 3)) * X + c8];
+        kv4_turn8(y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *(uint32_t*)(im + P::v_dword(4 * g, 8 * c8 + j)) = y[j];
       }
-      if (!is_v) {
-        uint8_t* o = page + P::k_byte(t0 + t, b);
-        *(u32x2*)o = u32x2{q[0], q[1]};
-        if (nd == 32) *(u32x2*)(o + 8) = u32x2{q[2], q[3]};
-        page[P::ks_byte(t0 + t, b)] = (uint8_t)sb;
+      wave_lds_fence();
+      if (n == 32) {
+#pragma unroll
+        for (int x = lane * 16; x < P::BYTES; x += 1024) *(u32x4*)(page + x) = *(const u32x4*)(im + x);
       } else {
+        for (int x = lane; x < n * X; x += 64) {
+          const int t = t0 + x / X, d = (x % X) * 8, o = P::k_byte(t, d >> 5) + ((d & 31) >> 1);
+          *(uint32_t*)(page + o) = *(const uint32_t*)(im + o);
+        }
+        for (int x = lane; x < n * 2 * P::NB; x += 64) {
+          const int t = t0 + x / (2 * P::NB), b = x % P::NB, o = x % (2 * P::NB) < P::NB ? P::ks_byte(t, b) : P::vs_byte(t, b);
+          page[o] = im[o];
+        }
+        for (int x = lane; x < 4 * D; x += 64) {
+          const int g = x / D;
+          uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) if (j < nd) vc[t0 + t][32 * b + j] = (uint8_t)((q[j >> 3] >> (4 * (j & 7))) & 15u);
-        page[P::vs_byte(t0 + t, b)] = (uint8_t)sb;
+          for (int j = 0; j < 8; ++j) { const int t = 16 * (j >> 2) + 4 * g + (j & 3); if (t >= t0 && t < t0 + n) mask |= 15u << (4 * j); }
+          uint32_t* o = (uint32_t*)(page + P::VOFF) + x;
+          const uint32_t val = *((const uint32_t*)(im + P::VOFF) + x);
+          if (mask == 0xffffffffu) *o = val;
+          else if (mask) { atomicAnd(o, ~mask); atomicOr(o, val & mask); }
+        }
       }
+      wave_lds_fence();
     }
-    __syncthreads();
-    for (int w2 = tid; w2 < 4 * D; w2 += 256) {
-      const int g = w2 / D, x = w2 - g * D, d = (x / P::NI) + 16 * (x % P::NI);
-      uint32_t val = 0, mask = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tt = 16 * (j >> 2) + 4 * g + (j & 3);
-        if (tt >= t0 && tt < t0 + n) { val |= (uint32_t)vc[tt][d] << (4 * j); mask |= 15u << (4 * j); }
-      }
-      uint32_t* o = (uint32_t*)(page + P::VOFF) + w2;
-      if (mask == 0xffffffffu) *o = val;
-      else if (mask) { atomicAnd(o, ~mask); atomicOr(o, val); }
-    }
-    __syncthreads();
     a += n;
   }
 }
@@ -109,7 +170,7 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
   if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
     return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_write: strides multiples of 8 elements, 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
-    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32), heads), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
+    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32), (heads + KV4_HEADS - 1) / KV4_HEADS), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
                        (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, slots, (long)tokens);
     return unimp_check_launch("kv4_write");
   });
@@ -184,40 +245,78 @@ extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_
 }
 
 // ------------------------------------------------------------------------------------------- read back as values
+// A wave per (run, head): every page is read once, whatever rows name its tokens.  K: a lane converts 8 dims of a token; V: a lane takes 8 tokens x 8 dims, turns the
+// nibbles round in registers and stores 16 bytes of each token.  Bound by the bf16 rows that leave.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, const int64_t* __restrict__ slots,
                                                        long tokens, bf16* __restrict__ k, bf16* __restrict__ v) {
   using P = Kv4<D>;
-  const long per = (long)heads * (D / 8), i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= tokens * per) return;
-  const long tok = i / per; const int r = (int)(i - tok * per), head = r / (D / 8), d = (r - head * (D / 8)) * 8;
-  const int64_t s = slots[tok];
-  bf16x8 ko = {}, vo = {};
-  if (s >= 0 && s < n_pages * KV4_PAGE) {
-    const uint8_t* page = pages + (long)blockIdx.y * layer_stride + ((s >> 5) * heads + head) * (long)P::BYTES;
-    const int t = (int)(s & 31), b = d >> 5, sh = 4 * kv4_nibble(t);
-    const uint32_t kc = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1));
-    const float ks = kv4_scale(page[P::ks_byte(t, b)]), vs = kv4_scale(page[P::vs_byte(t, b)]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ko[j] = f2bf(kv4_value((kc >> (4 * j)) & 15u) * ks);
-      vo[j] = f2bf(kv4_value((*(const uint32_t*)(page + P::v_dword(t, d + j)) >> sh) & 15u) * vs);
+  constexpr int X = D / 8;
+  __shared__ int64_t sl[65];
+  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const long i0 = (long)blockIdx.x * 32;
+  kv4_load_slots(sl, slots, i0, tokens, n_pages);
+  const long lo = (long)blockIdx.z * tokens;
+  const int h0 = blockIdx.y * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
+  auto bf16s = [](uint32_t c, uint32_t byte) {                       // eight codes as values
+    const float sc = kv4_scale(byte);
+    union { bf16x2 h[4]; bf16x8 v; } u;
+    u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0); u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1);
+    u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2); u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3);
+    if (byte == 255u) { const uint32_t nn = 0x7fc07fc0u; u.h[0] = u.h[1] = u.h[2] = u.h[3] = __builtin_bit_cast(bf16x2, nn); }
+    return u.v;
+  };
+  for (int a = 0; a < 32 && i0 + a < tokens;) {
+    const int64_t s0 = sl[a + 1];
+    if (s0 < 0) {                                                    // no slot: zeros
+      for (int x = threadIdx.x; x < (h1 - h0) * X; x += 256) {
+        const long o = ((lo + i0 + a) * heads + h0) * D + 8 * x;
+        *(bf16x8*)(k + o) = bf16x8{}; *(bf16x8*)(v + o) = bf16x8{};
+      }
+      ++a; continue;
     }
+    const int n = kv4_run(sl, a);
+    if (!n) { ++a; continue; }                                       // the previous chunk's
+    const int t0 = (int)(s0 & 31);
+    for (int head = h0 + w; head < h1; head += 4) {
+      const uint8_t* page = pages + (long)blockIdx.z * layer_stride + ((s0 >> 5) * heads + head) * (long)P::BYTES;
+      const long row0 = lo + i0 + a - t0;                            // output row of the page's token 0
+#pragma unroll
+      for (int x = lane; x < 32 * X; x += 64) {
+        const int t = x / X, d = (x - t * X) * 8, b = d >> 5;
+        if (t >= t0 && t < t0 + n) {
+          const uint32_t c = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1));
+          *(bf16x8*)(k + ((row0 + t) * heads + head) * D + d) = bf16s(c, page[P::ks_byte(t, b)]);
+        }
+      }
+      for (int x = lane; x < 4 * X; x += 64) {
+        const int g = x / X, d = (x - g * X) * 8;
+        uint32_t y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = *(const uint32_t*)(page + P::v_dword(4 * g, d + j));
+        const u32x2 sc = *(const u32x2*)(page + P::VS + 8 * P::NB * g + 8 * (d >> 5));
+        kv4_turn8(y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = 16 * (j >> 2) + 4 * g + (j & 3);
+          if (t >= t0 && t < t0 + n) *(bf16x8*)(v + ((row0 + t) * heads + head) * D + d) = bf16s(y[j], (sc[j >> 2] >> (8 * (j & 3))) & 0xffu);
+        }
+      }
+    }
+    a += n;
   }
-  const long o = (((long)blockIdx.y * tokens + tok) * heads + head) * D + d;
-  *(bf16x8*)(k + o) = ko; *(bf16x8*)(v + o) = vo;
 }
 
 extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, const int64_t* slots, int64_t tokens, void* k,
                               void* v, void* stream) {
   if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
-  if (layers > 65535 || tokens > (int64_t)1 << 28 || tokens * heads * hd > (int64_t)1 << 34)
-    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and 2^34 elements of a layer");
+  if (layers > 65535 || heads > 65535 || tokens > (int64_t)1 << 28)
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^28 tokens");
   if (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_read: 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens * heads * (D / 8) + 255) / 256), layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
+    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens + 31) / 32), (heads + KV4_HEADS - 1) / KV4_HEADS, layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
                        (long)layer_stride, (long)n_pages, heads, slots, (long)tokens, (bf16*)k, (bf16*)v);
     return unimp_check_launch("kv4_read");
   });
