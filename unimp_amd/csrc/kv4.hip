@@ -38,6 +38,9 @@ __device__ __forceinline__ int kv4_run(const int64_t (&sl)[65], int a) {
   const bool on = lane < 32 && a + lane < 64 && t0 + lane < 32 && sl[min(a + 1 + lane, 64)] == s0 + lane;      // lane 0: itself
   return __builtin_ctzll(~__ballot(on));
 }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
 // eight dwords of eight nibbles, turned round: out[i] nibble j = in[j] nibble i
 __device__ __forceinline__ void kv4_turn8(uint32_t (&x)[8]) {
 #pragma unroll
@@ -67,40 +70,45 @@ __device__ __forceinline__ void wave_lds_fence() {                   // LDS of t
 // A wave per (run, head).  Four lanes hold an MX block of a token (16-byte loads, the block's maximum by two lane exchanges); V's codes turn round (8 tokens x 8 dims
 // per lane) through LDS; the page is put together in LDS and leaves in 16-byte stores.  A run that does not fill its page writes its own bytes, and its nibbles of V dwords
 // that other runs share by atomic and + or: the fields are disjoint, the result does not depend on the order.
-#define KV4_HEADS 8                                                  // heads of a workgroup
+#define KV4_HEADS 8                                                  // heads of a workgroup; the head blocks of a chunk are neighbours in the grid (whole rows in flight)
 template <int D>
-__global__ __launch_bounds__(256) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
-                                                        uint8_t* __restrict__ pages, long n_pages, int heads, const int64_t* __restrict__ slots, long tokens) {
+__global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
+                                                           uint8_t* __restrict__ pages, long n_pages, int heads, int head_blocks, const int64_t* __restrict__ slots, long tokens) {
   using P = Kv4<D>;
-  constexpr int PASSES = 2 * P::NB, X = D / 8;                       // (token, block) pairs in sixteens; 8-dim pieces of a row
+  constexpr int X = D / 8, TP = 16 / P::NB, PASSES = (32 + TP - 1) / TP;      // 8-dim pieces of a row; tokens of a pass (four lanes to a block)
   __shared__ int64_t sl[65];
   __shared__ __attribute__((aligned(16))) uint8_t image[4][P::BYTES];
   __shared__ uint32_t turn[4][32 * X];
-  const int lane = lane_id(), w = threadIdx.x >> 6, quad = lane & 3;
-  const long i0 = (long)blockIdx.x * 32;
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane & 3;
+  const int tl = (lane >> 2) / P::NB, b = (lane >> 2) - tl * P::NB, d = 32 * b + 8 * quad;      // this lane's token of a pass, block and dims
+  const bool on = tl < TP && d < D;
+  const long chunk = blockIdx.x / head_blocks, i0 = chunk * 32;
+  const int h0 = (blockIdx.x - (unsigned)chunk * head_blocks) * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
   kv4_load_slots(sl, slots, i0, tokens, n_pages);
   uint8_t* im = image[w];
   uint32_t* tv = turn[w];
   for (int a = 0; a < 32;) {
-    const int n = kv4_run(sl, a);
+    const int n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
     if (!n) { ++a; continue; }                                       // no slot, or the tail of the previous chunk's last run
-    const int64_t s0 = sl[a + 1];
+    const int64_t s0 = uniform64(sl[a + 1]);
     const int t0 = (int)(s0 & 31);
-    for (int head = blockIdx.y * KV4_HEADS + w; head < min((int)(blockIdx.y + 1) * KV4_HEADS, heads); head += 4) {
+    const long row0 = i0 + a - t0;                                   // the row that page token 0 has or would have
+    for (int head = h0 + w; head < h1; head += 4) {
       uint8_t* page = pages + ((s0 >> 5) * heads + head) * (long)P::BYTES;
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
+        const bf16* src = kind ? v + head * v_hs : k + head * k_hs;
+        const long ts = kind ? v_ts : k_ts;
         bf16x8 u[PASSES];
 #pragma unroll
         for (int ps = 0; ps < PASSES; ++ps) {                        // all loads of the half page first
-          const int pr = ps * 16 + (lane >> 2), t = pr / P::NB, b = pr - t * P::NB, d = 32 * b + 8 * quad;
+          const int t = ps * TP + tl;
           u[ps] = bf16x8{};
-          if (t >= t0 && t < t0 + n && d < D)
-            u[ps] = *(const bf16x8*)(kind ? v + (i0 + a + t - t0) * v_ts + head * v_hs + d : k + (i0 + a + t - t0) * k_ts + head * k_hs + d);
+          if (on && t >= t0 && t < t0 + n) u[ps] = *(const bf16x8*)(src + (row0 + t) * ts + d);
         }
 #pragma unroll
         for (int ps = 0; ps < PASSES; ++ps) {
-          const int pr = ps * 16 + (lane >> 2), t = pr / P::NB, b = pr - t * P::NB, d = 32 * b + 8 * quad;
+          const int t = ps * TP + tl;
           float f[8];
           uint32_t m = 0;
 #pragma unroll
@@ -115,16 +123,16 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const bf16* __restrict__
           r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[4], f[5], scale, 2);
           r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[6], f[7], scale, 3);
           if (sb == 255) r = 0;
-          if (d < D) {
+          if (on && t < 32) {
             if (!kind) *(uint32_t*)(im + P::k_byte(t, b) + 4 * quad) = r;
             else tv[t * X + (d >> 3)] = r;
+            if (!quad) im[kind ? P::vs_byte(t, b) : P::ks_byte(t, b)] = (uint8_t)sb;
           }
-          if (!quad) im[kind ? P::vs_byte(t, b) : P::ks_byte(t, b)] = (uint8_t)sb;
         }
       }
       wave_lds_fence();
-      for (int x = lane; x < 4 * X; x += 64) {                       // lane: 8 tokens of group g, 8 dims
-        const int g = x / X, c8 = x - g * X;
+      if (4 * X == 64 || lane < 4 * X) {                             // lane: 8 tokens of group g, 8 dims
+        const int g = lane / X, c8 = lane - g * X;
         uint32_t y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = tv[(16 * (j >> 2) + 4 * g + (j & 3)) * X + c8];
@@ -138,11 +146,11 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const bf16* __restrict__
         for (int x = lane * 16; x < P::BYTES; x += 1024) *(u32x4*)(page + x) = *(const u32x4*)(im + x);
       } else {
         for (int x = lane; x < n * X; x += 64) {
-          const int t = t0 + x / X, d = (x % X) * 8, o = P::k_byte(t, d >> 5) + ((d & 31) >> 1);
+          const int t = t0 + x / X, c = (x % X) * 8, o = P::k_byte(t, c >> 5) + ((c & 31) >> 1);
           *(uint32_t*)(page + o) = *(const uint32_t*)(im + o);
         }
         for (int x = lane; x < n * 2 * P::NB; x += 64) {
-          const int t = t0 + x / (2 * P::NB), b = x % P::NB, o = x % (2 * P::NB) < P::NB ? P::ks_byte(t, b) : P::vs_byte(t, b);
+          const int t = t0 + x / (2 * P::NB), bb = x % P::NB, o = x % (2 * P::NB) < P::NB ? P::ks_byte(t, bb) : P::vs_byte(t, bb);
           page[o] = im[o];
         }
         for (int x = lane; x < 4 * D; x += 64) {
@@ -166,12 +174,13 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
                                int hd, const int64_t* slots, int64_t tokens, void* stream) {
   if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
   if (tokens <= 0 || heads <= 0 || n_pages <= 0) return UNIMP_OK;
-  if (heads > 65535 || tokens > (int64_t)1 << 28) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^28 tokens");
+  const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
+  if (heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^31 token heads");
   if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
     return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_write: strides multiples of 8 elements, 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
-    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32), (heads + KV4_HEADS - 1) / KV4_HEADS), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
-                       (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, slots, (long)tokens);
+    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32 * hb)), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
+                       (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, (int)hb, slots, (long)tokens);
     return unimp_check_launch("kv4_write");
   });
 }
@@ -248,17 +257,19 @@ extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_
 // A wave per (run, head): every page is read once, whatever rows name its tokens.  K: a lane converts 8 dims of a token; V: a lane takes 8 tokens x 8 dims, turns the
 // nibbles round in registers and stores 16 bytes of each token.  Bound by the bf16 rows that leave.
 template <int D>
-__global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, const int64_t* __restrict__ slots,
-                                                       long tokens, bf16* __restrict__ k, bf16* __restrict__ v) {
+__global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, int head_blocks,
+                                                          const int64_t* __restrict__ slots, long tokens, bf16* __restrict__ k, bf16* __restrict__ v) {
   using P = Kv4<D>;
-  constexpr int X = D / 8;
+  constexpr int X = D / 8, TP = 64 / X, PASSES = (32 + TP - 1) / TP;          // 8-dim pieces of a row; tokens of a pass
   __shared__ int64_t sl[65];
-  const int lane = lane_id(), w = threadIdx.x >> 6;
-  const long i0 = (long)blockIdx.x * 32;
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tl = lane / X, d = (lane - tl * X) * 8, b = d >> 5;               // K: this lane's token of a pass and dims; V: tl = group g of 8 tokens
+  const long chunk = blockIdx.x / head_blocks, i0 = chunk * 32;
+  const int h0 = (blockIdx.x - (unsigned)chunk * head_blocks) * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
   kv4_load_slots(sl, slots, i0, tokens, n_pages);
-  const long lo = (long)blockIdx.z * tokens;
-  const int h0 = blockIdx.y * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
-  auto bf16s = [](uint32_t c, uint32_t byte) {                       // eight codes as values
+  const long lo = (long)blockIdx.y * tokens;
+  const long row = (long)heads * D;                                            // elements of an output row
+  auto values = [](uint32_t c, uint32_t byte) {                                // eight codes as values
     const float sc = kv4_scale(byte);
     union { bf16x2 h[4]; bf16x8 v; } u;
     u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0); u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1);
@@ -267,39 +278,44 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict
     return u.v;
   };
   for (int a = 0; a < 32 && i0 + a < tokens;) {
-    const int64_t s0 = sl[a + 1];
+    const int64_t s0 = uniform64(sl[a + 1]);
     if (s0 < 0) {                                                    // no slot: zeros
       for (int x = threadIdx.x; x < (h1 - h0) * X; x += 256) {
-        const long o = ((lo + i0 + a) * heads + h0) * D + 8 * x;
+        const long o = (lo + i0 + a) * row + h0 * D + 8 * x;
         *(bf16x8*)(k + o) = bf16x8{}; *(bf16x8*)(v + o) = bf16x8{};
       }
       ++a; continue;
     }
-    const int n = kv4_run(sl, a);
+    const int n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
     if (!n) { ++a; continue; }                                       // the previous chunk's
     const int t0 = (int)(s0 & 31);
     for (int head = h0 + w; head < h1; head += 4) {
-      const uint8_t* page = pages + (long)blockIdx.z * layer_stride + ((s0 >> 5) * heads + head) * (long)P::BYTES;
-      const long row0 = lo + i0 + a - t0;                            // output row of the page's token 0
+      const uint8_t* page = pages + (long)blockIdx.y * layer_stride + ((s0 >> 5) * heads + head) * (long)P::BYTES;
+      const long o0 = (lo + i0 + a - t0) * row + head * D;           // output of the page's token 0
+      uint32_t c[PASSES], ks[PASSES], y[8];
+      u32x2 vs = {0, 0};
 #pragma unroll
-      for (int x = lane; x < 32 * X; x += 64) {
-        const int t = x / X, d = (x - t * X) * 8, b = d >> 5;
-        if (t >= t0 && t < t0 + n) {
-          const uint32_t c = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1));
-          *(bf16x8*)(k + ((row0 + t) * heads + head) * D + d) = bf16s(c, page[P::ks_byte(t, b)]);
-        }
+      for (int ps = 0; ps < PASSES; ++ps) {                          // the page's loads first
+        const int t = ps * TP + tl;
+        c[ps] = ks[ps] = 0;
+        if (tl < TP && t < 32) { c[ps] = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1)); ks[ps] = page[P::ks_byte(t, b)]; }
       }
-      for (int x = lane; x < 4 * X; x += 64) {
-        const int g = x / X, d = (x - g * X) * 8;
-        uint32_t y[8];
+      if (tl < 4) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = *(const uint32_t*)(page + P::v_dword(4 * g, d + j));
-        const u32x2 sc = *(const u32x2*)(page + P::VS + 8 * P::NB * g + 8 * (d >> 5));
+        for (int j = 0; j < 8; ++j) y[j] = *(const uint32_t*)(page + P::v_dword(4 * tl, d) + 4 * P::NI * j);
+        vs = *(const u32x2*)(page + P::VS + 8 * P::NB * tl + 8 * b);
+      }
+#pragma unroll
+      for (int ps = 0; ps < PASSES; ++ps) {
+        const int t = ps * TP + tl;
+        if (tl < TP && t >= t0 && t < t0 + n) *(bf16x8*)(k + o0 + ps * TP * row + (tl * (int)row + d)) = values(c[ps], ks[ps]);
+      }
+      if (tl < 4) {
         kv4_turn8(y);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = 16 * (j >> 2) + 4 * g + (j & 3);
-          if (t >= t0 && t < t0 + n) *(bf16x8*)(v + ((row0 + t) * heads + head) * D + d) = bf16s(y[j], (sc[j >> 2] >> (8 * (j & 3))) & 0xffu);
+          const int t = 16 * (j >> 2) + 4 * tl + (j & 3);
+          if (t >= t0 && t < t0 + n) *(bf16x8*)(v + o0 + (16 * (j >> 2) + (j & 3)) * row + (4 * tl * (int)row + d)) = values(y[j], (vs[j >> 2] >> (8 * (j & 3))) & 0xffu);
         }
       }
     }
@@ -311,13 +327,14 @@ extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layer
                               void* v, void* stream) {
   if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
-  if (layers > 65535 || heads > 65535 || tokens > (int64_t)1 << 28)
-    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^28 tokens");
+  const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
+  if (layers > 65535 || heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23)
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^31 token heads");
   if (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_read: 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens + 31) / 32), (heads + KV4_HEADS - 1) / KV4_HEADS, layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
-                       (long)layer_stride, (long)n_pages, heads, slots, (long)tokens, (bf16*)k, (bf16*)v);
+    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens + 31) / 32 * hb), layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
+                       (long)layer_stride, (long)n_pages, heads, (int)hb, slots, (long)tokens, (bf16*)k, (bf16*)v);
     return unimp_check_launch("kv4_read");
   });
 }
