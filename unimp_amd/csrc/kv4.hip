@@ -70,7 +70,7 @@ __device__ __forceinline__ void wave_lds_fence() {                   // LDS of t
 // A wave per (run, head).  Four lanes hold an MX block of a token (16-byte loads, the block's maximum by two lane exchanges); V's codes turn round (8 tokens x 8 dims
 // per lane) through LDS; the page is put together in LDS and leaves in 16-byte stores.  A run that does not fill its page writes its own bytes, and its nibbles of V dwords
 // that other runs share by atomic and + or: the fields are disjoint, the result does not depend on the order.
-#define KV4_HEADS 8                                                  // heads of a workgroup; the head blocks of a chunk are neighbours in the grid (whole rows in flight)
+#define KV4_HEADS 4                                                  // heads of a workgroup; the head blocks of a chunk are neighbours in the grid (whole rows in flight)
 template <int D>
 __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
                                                            uint8_t* __restrict__ pages, long n_pages, int heads, int head_blocks, const int64_t* __restrict__ slots, long tokens) {
@@ -82,6 +82,7 @@ __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restric
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane & 3;
   const int tl = (lane >> 2) / P::NB, b = (lane >> 2) - tl * P::NB, d = 32 * b + 8 * quad;      // this lane's token of a pass, block and dims
   const bool on = tl < TP && d < D;
+  const long lane_k = tl * k_ts + d, lane_v = tl * v_ts + d;
   const long chunk = blockIdx.x / head_blocks, i0 = chunk * 32;
   const int h0 = (blockIdx.x - (unsigned)chunk * head_blocks) * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
   kv4_load_slots(sl, slots, i0, tokens, n_pages);
@@ -97,14 +98,15 @@ __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restric
       uint8_t* page = pages + ((s0 >> 5) * heads + head) * (long)P::BYTES;
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        const bf16* src = kind ? v + head * v_hs : k + head * k_hs;
         const long ts = kind ? v_ts : k_ts;
+        const bf16* src = (kind ? v + head * v_hs : k + head * k_hs) + row0 * ts;
+        const bf16* mine = src + (kind ? lane_v : lane_k);
         bf16x8 u[PASSES];
 #pragma unroll
         for (int ps = 0; ps < PASSES; ++ps) {                        // all loads of the half page first
           const int t = ps * TP + tl;
           u[ps] = bf16x8{};
-          if (on && t >= t0 && t < t0 + n) u[ps] = *(const bf16x8*)(src + (row0 + t) * ts + d);
+          if (on && t >= t0 && t < t0 + n) u[ps] = *(const bf16x8*)(mine + ps * TP * ts);
         }
 #pragma unroll
         for (int ps = 0; ps < PASSES; ++ps) {
@@ -279,12 +281,14 @@ __global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restr
   };
   for (int a = 0; a < 32 && i0 + a < tokens;) {
     const int64_t s0 = uniform64(sl[a + 1]);
-    if (s0 < 0) {                                                    // no slot: zeros
-      for (int x = threadIdx.x; x < (h1 - h0) * X; x += 256) {
-        const long o = (lo + i0 + a) * row + h0 * D + 8 * x;
+    if (s0 < 0) {                                                    // no slots: rows of zeros, up to the next slot
+      const int end = (int)min(32l, tokens - i0);
+      const int z = __builtin_ctzll(~__ballot(lane < 32 && a + lane < end && sl[min(a + 1 + lane, 64)] < 0)), per = (h1 - h0) * X;
+      for (int x = threadIdx.x; x < z * per; x += 256) {
+        const long o = (lo + i0 + a + x / per) * row + h0 * D + 8 * (x % per);
         *(bf16x8*)(k + o) = bf16x8{}; *(bf16x8*)(v + o) = bf16x8{};
       }
-      ++a; continue;
+      a += z; continue;
     }
     const int n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
     if (!n) { ++a; continue; }                                       // the previous chunk's
