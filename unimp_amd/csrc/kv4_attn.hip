@@ -105,9 +105,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
       const int d0 = 64 * h + 16 * g;
       float x[16];
       uint32_t mx = 0;
+      const bool in = qi < nq && d0 < D;                                          // 16 dims are inside the head or behind it
+      const bf16x8 u0 = in ? *(const bf16x8*)(qp + d0) : bf16x8{}, u1 = in ? *(const bf16x8*)(qp + d0 + 8) : bf16x8{};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        x[j] = qi < nq && d0 + j < D ? bf2f(qp[d0 + j]) : 0.f;
+        x[j] = bf2f(j < 8 ? u0[j & 7] : u1[j & 7]);
         mx = max(mx, __float_as_uint(x[j]) & 0x7fffffffu);
       }
       mx = max(mx, __shfl_xor(mx, 16, 64));                                       // the other half of the 32-dim block
@@ -340,7 +342,8 @@ static int kv4_attn_check(const unimp_kv4_attn_desc* d) {
       d->heads > 65535 || d->n_pages <= 0)
     return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 32767 rows, 2^26 pages of a row; a pool with pages");
   if (d->hd != 64 && d->hd != 80 && d->hd != 128) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
-  if ((uintptr_t)d->pages & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_attn_decode: 16-byte aligned pages");
+  if ((((uintptr_t)d->pages | (uintptr_t)d->q) & 15) || ((d->q_row_stride | d->q_head_stride) & 7))
+    return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_attn_decode: 16-byte aligned pages and q, q strides multiples of 8 elements");
   return UNIMP_OK;
 }
 

@@ -1221,6 +1221,7 @@ def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_l
         out = torch.empty((rows, heads, hd), dtype=bf16, device=q.device)
     _need(out.dtype == bf16 and out.shape == q.shape and out.stride(2) == 1, "out: bf16 like q, unit dim stride")
     _same_device(pages, q, tables, lens, alibi, shared_len, out)
+    q = _kv4_rows(q, hd)
     d = _lib.Kv4AttnDesc()
     d.q, d.q_row_stride, d.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
     d.pages, d.n_pages, d.kv_heads, d.hd = pages.data_ptr(), n_pages, kv_heads, hd
