@@ -20,7 +20,7 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
   int rows, heads; float scale; const float* alibi; bf16* o; long o_rs, o_hs; int group; const int32_t* shared;
-  int chunk, slots;                    // pages of a workgroup; partial slots per row and part (prefix / rest)
+  int G, chunk, slots;                 // query heads of a key head; pages of a workgroup; partial slots per row and part (prefix / rest)
   float* ws;                           // null: a workgroup holds a row's whole range and writes o
 };
 
@@ -40,76 +40,85 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int NI = P::NI;
   __shared__ float so[NW][CO::Q][D], sm[NW][CO::Q], sl[NW][CO::Q];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, G = a.heads / a.kv_heads;
+  const int kvh = blockIdx.y, G = a.G;
   // ---- which rows and columns of their tables: z < rows: the row's own pages; above: the pages that a group shares, for all its queries at once
   const bool prefix = (int)blockIdx.z >= a.rows;
   const int row = prefix ? ((int)blockIdx.z - a.rows) * a.group : (int)blockIdx.z;
   const int nq = prefix ? a.group * G : G;
-  const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
   const int qi = col / CO::VAR, var = col % CO::VAR;
   const int my_row = prefix ? row + min(qi / G, a.group - 1) : row, my_head = kvh * G + (qi < nq ? qi % G : 0);
-  const int my_len = min(max(a.lens[my_row], 0), a.width * KV4_PAGE);
-  int top = my_len;                                                               // the longest of the rows here
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 16));
-  top = __builtin_amdgcn_readfirstlane(top);
-  const int cols = (top + KV4_PAGE - 1) / KV4_PAGE;
-  const int first = prefix ? 0 : min(shared, cols), last = prefix ? min(shared, cols) : cols;
-  const int c0 = first + blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, last);
-  if (c0 >= c1 && !(a.ws == nullptr)) return;                                     // nothing here (a row without tokens still gets its zeros)
 
-  // ---- page ids of this wave: page c0 + w + NW k in lane k
-  const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;
-  int ids = -1;
-  if (lane < n) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
-  if (ids >= a.n_pages) ids = -1;
-
-  auto load = [&](Kv4Frag<D>& f, int k) {
-    const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
-    const uint8_t* page = a.pages + ((long)id * a.kv_heads + kvh) * P::BYTES;
-    const u32x4 z = {0, 0, 0, 0};
+  // queries: lane (c, g) holds dims 16 g ... and 64 + 16 g ... of column c's query (16 dims are inside the head or behind it).  Requested first: what is waited for in
+  // order must not stand behind the pages.
+  bf16x8 qu[4];
+  {
+    const bf16* qp = a.q + (long)my_row * a.q_rs + (long)my_head * a.q_hs;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      f.k[h] = z;
-      if (D == 128 || g < P::NB - (P::BLK_LAST < 32)) f.k[h] = *(const u32x4*)(page + 512 * g + (16 * h + col) * 16);
-      else if (P::BLK_LAST < 32 && g == P::NB - 1) { const u32x2 t = *(const u32x2*)(page + 512 * g + (16 * h + col) * 8); f.k[h] = u32x4{t[0], t[1], 0, 0}; }
+      const bool in = qi < nq && 64 * h + 16 * g < D;
+      qu[2 * h] = in ? *(const bf16x8*)(qp + 64 * h + 16 * g) : bf16x8{};
+      qu[2 * h + 1] = in ? *(const bf16x8*)(qp + 64 * h + 16 * g + 8) : bf16x8{};
+    }
+  }
+  const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
+  const int c0 = (prefix ? 0 : shared) + blockIdx.x * a.chunk;
+  // page ids of this wave: page c0 + w + NW k in lane k; requested beside the lengths
+  int ids = -1;
+  if (NW * lane + w < a.chunk && c0 + w + NW * lane < a.width) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
+  const int my_len = min(max(a.lens[my_row], 0), a.width * KV4_PAGE);
+  int top = my_len;                                                               // the longest of the rows here
+  if (prefix) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 16));
+  }
+  top = __builtin_amdgcn_readfirstlane(top);
+  const int cols = (top + KV4_PAGE - 1) / KV4_PAGE;
+  const int c1 = min(c0 + a.chunk, prefix ? min(shared, cols) : cols);
+  if (c0 >= c1 && a.ws) return;                                                   // nothing here (a row without tokens still gets its zeros)
+  const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;                    // pages of this wave
+  if (ids >= a.n_pages) ids = -1;
+
+  const uint32_t k_at = P::BLK_LAST < 32 && g == P::NB - 1 ? 512 * g + 8 * col : 512 * g + 16 * col, ks_at = P::KS + 32 * g + 2 * col;
+  const uint32_t v_at = P::VOFF + 4 * (g * D + col * NI), vs_at = P::VS + 8 * P::NB * g + (MODE == 2 ? 0 : 8 * min(MODE == 0 ? var >> 1 : var, P::NB - 1));
+  auto page_of = [&](int k) { return a.pages + ((long)max(__builtin_amdgcn_readlane(ids, k), 0) * a.kv_heads + kvh) * P::BYTES; };
+  // every lane's loads of page k, unconditional (past the last page: that one again, from the cache), so that the number in flight is known everywhere
+  auto load = [&](Kv4Frag<D>& f, int k) {
+    const uint8_t* page = page_of(min(k, n - 1));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (D == 128) f.k[h] = *(const u32x4*)(page + k_at + 256 * h);
+      else {
+        f.k[h] = u32x4{0, 0, 0, 0};
+        if (g < P::NB - (P::BLK_LAST < 32)) f.k[h] = *(const u32x4*)(page + k_at + 256 * h);
+        else if (P::BLK_LAST < 32 && g == P::NB - 1) { const u32x2 t = *(const u32x2*)(page + k_at + 128 * h); f.k[h] = u32x4{t[0], t[1], 0, 0}; }
+      }
     }
     f.ks = 0x7f7f;
-    if (D == 128 || g < P::NB) f.ks = *(const uint16_t*)(page + P::KS + 32 * g + 2 * col);
-    const uint8_t* vp = page + P::VOFF + 4 * (g * D + col * NI);
+    if (D == 128 || g < P::NB) f.ks = *(const uint16_t*)(page + ks_at);
     if constexpr (D == 80) {
       typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4u;
-      f.v0 = *(const u32x4u*)vp; f.v1[0] = *(const uint32_t*)(vp + 16);
+      f.v0 = *(const u32x4u*)(page + v_at); f.v1[0] = *(const uint32_t*)(page + v_at + 16);
     } else {
-      f.v0 = *(const u32x4*)vp;
-      if (D == 128) f.v1 = *(const u32x4*)(vp + 16);
+      f.v0 = *(const u32x4*)(page + v_at);
+      if (D == 128) f.v1 = *(const u32x4*)(page + v_at + 16);
     }
-    if constexpr (MODE < 2) {
-      const int b = min(MODE == 0 ? var >> 1 : var, P::NB - 1);
-      f.vs = *(const u32x2*)(page + P::VS + 8 * P::NB * g + 8 * b);
-    }
+    if constexpr (MODE < 2) f.vs = *(const u32x2*)(page + vs_at);
   };
 
   Kv4Frag<D> fa, fb;
-  if (n > 0) load(fa, 0);
-  if (n > 1) load(fb, 1);
+  if (n > 0) { load(fa, 0); load(fb, 1); }
 
-  // ---- queries: lane (c, g) holds dims 16 g ... and 64 + 16 g ... of column c's query
   i32x8 qh, ql;
   int sb;
   {
-    const bf16* qp = a.q + (long)my_row * a.q_rs + (long)my_head * a.q_hs;
     int sx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int d0 = 64 * h + 16 * g;
       float x[16];
       uint32_t mx = 0;
-      const bool in = qi < nq && d0 < D;                                          // 16 dims are inside the head or behind it
-      const bf16x8 u0 = in ? *(const bf16x8*)(qp + d0) : bf16x8{}, u1 = in ? *(const bf16x8*)(qp + d0 + 8) : bf16x8{};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        x[j] = bf2f(j < 8 ? u0[j & 7] : u1[j & 7]);
+        x[j] = bf2f(qu[2 * h + (j >> 3)][j & 7]);
         mx = max(mx, __float_as_uint(x[j]) & 0x7fffffffu);
       }
       mx = max(mx, __shfl_xor(mx, 16, 64));                                       // the other half of the 32-dim block
@@ -161,8 +170,10 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
     const bool part = __any(vis < KV4_PAGE);
     if (part) {                                                                   // the last page, or a hidden one
+      int g4 = 4 * g;
+      asm volatile("" : "+v"(g4));                                                // keeps these comparisons from living in registers across the loop
 #pragma unroll
-      for (int j = 0; j < 8; ++j) if (16 * (j >> 2) + 4 * g + (j & 3) >= vis) x[j] = -INFINITY;
+      for (int j = 0; j < 8; ++j) if (16 * (j >> 2) + g4 + (j & 3) >= vis) x[j] = -INFINITY;
     }
     const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (__any(mx > m + 10.f)) {
@@ -199,11 +210,8 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
     union B { uint32_t d[4]; bf16x8 v; };
     auto hide = [&](uint32_t& d0, uint32_t& d1) {                                 // scale bytes of tokens that are not there: 0, whatever memory holds
       if (part) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (4 * g + j >= vis) d0 &= ~(0xffu << (8 * j));
-          if (16 + 4 * g + j >= vis) d1 &= ~(0xffu << (8 * j));
-        }
+        const int n0 = min(max(vis - 4 * g, 0), 4), n1 = min(max(vis - 16 - 4 * g, 0), 4);      // of four
+        d0 &= (uint32_t)((1ull << (8 * n0)) - 1); d1 &= (uint32_t)((1ull << (8 * n1)) - 1);
       }
     };
     if constexpr (MODE == 0) {
@@ -228,8 +236,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
     } else {
-      const int id = max(__builtin_amdgcn_readlane(ids, k), 0);
-      const uint8_t* sp = a.pages + ((long)id * a.kv_heads + kvh) * P::BYTES + P::VS + 8 * P::NB * g;
+      const uint8_t* sp = page_of(k) + vs_at;
 #pragma unroll
       for (int blk = 0; blk < P::NB; ++blk) {
         const u32x2 d = *(const u32x2*)(sp + 8 * blk);
@@ -248,14 +255,13 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
   };
 
-  for (int k = 0; k < n; k += 2) {
+  for (int k = 0; k + 1 < n; k += 2) {
     compute(fa, k);
-    if (k + 2 < n) load(fa, k + 2);
-    if (k + 1 < n) {
-      compute(fb, k + 1);
-      if (k + 3 < n) load(fb, k + 3);
-    }
+    load(fa, k + 2);
+    compute(fb, k + 1);
+    load(fb, k + 3);
   }
+  if (n & 1) compute(fa, n - 1);
 
   // ---- join the waves: lane (c, g) holds dims 16 i + 4 g + e of column c
   l += __shfl_xor(l, 16, 64);
@@ -330,7 +336,7 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   p.mode = nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : 2;
   const long units = (long)d->rows * d->kv_heads;
   p.nw = p.mode < 2 && units < 512 ? 8 : 4;
-  const long want = (long)d->width * units / 2048;                                // pages of a workgroup that leave 2048 workgroups
+  const long want = (long)d->width * units / 1024;                                // pages of a workgroup that leave 1024 workgroups
   p.chunk = (int)(want < 4 * p.nw ? 4 * p.nw : want > 32 * p.nw ? 32 * p.nw : want);
   p.slots = d->width > 0 ? (d->width + p.chunk - 1) / p.chunk : 1;
   p.floats = p.group == 1 && p.slots == 1 ? 0 : (int64_t)units * G * (p.group > 1 ? 2 : 1) * p.slots * (d->hd + 2);
@@ -373,7 +379,7 @@ extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* worksp
   const Kv4Plan p = kv4_plan(d);
   if (p.floats && !workspace) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: workspace of unimp_kv4_attn_workspace floats");
   Kv4AttnArgs a{(const bf16*)d->q, d->q_row_stride, d->q_head_stride, (const uint8_t*)d->pages, d->n_pages, d->kv_heads, d->tables, d->table_stride, d->width, d->lens,
-                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, p.group, d->shared_len, p.chunk, p.slots,
+                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, p.group, d->shared_len, d->heads / d->kv_heads, p.chunk, p.slots,
                 p.floats ? workspace : nullptr};
   switch (d->hd) {
     case 64: kv4_attn_launch<64>(a, p, (hipStream_t)stream); break;
