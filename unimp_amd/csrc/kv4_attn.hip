@@ -20,7 +20,8 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
   int rows, heads; float scale; const float* alibi; bf16* o; long o_rs, o_hs; int group; const int32_t* shared;
-  int G, chunk, slots;                 // query heads of a key head; pages of a workgroup; partial slots per row and part (prefix / rest)
+  int G, chunk, slots;                 // query heads of a key head; pages of a workgroup on a row's own columns; its partial slots
+  int chunk_p, slots_p;                // the same for the columns that a group shares (slots_p = 0: no groups)
   float* ws;                           // null: a workgroup holds a row's whole range and writes o
 };
 
@@ -33,17 +34,21 @@ template <int D> struct Kv4Frag {        // one page as a wave holds it
   u32x4 k[2]; u32x4 v0; u32x4 v1; uint32_t ks; u32x2 vs;
 };
 
-template <int D, int MODE, int NW, bool ALIBI>
-__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
+// slot i of a (row, head) in the workspace: [0, slots_p) the group's columns, then the row's own; hd sums, maximum, sum of exponentials
+__device__ __forceinline__ float* kv4_partial(const Kv4AttnArgs& a, int D, int row, int head, int slot) {
+  return a.ws + (((long)row * a.heads + head) * (a.slots_p + a.slots) + slot) * (D + 2);
+}
+
+// prefix: the columns that a group's rows share, for the queries of all of them; else one row's own columns
+template <int D, int MODE, int NW, bool ALIBI, bool prefix>
+__device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   using P = Kv4<D>;
   using CO = Kv4Cols<D, MODE>;
   constexpr int NI = P::NI;
   __shared__ float so[NW][CO::Q][D], sm[NW][CO::Q], sl[NW][CO::Q];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, G = a.G;
-  // ---- which rows and columns of their tables: z < rows: the row's own pages; above: the pages that a group shares, for all its queries at once
-  const bool prefix = (int)blockIdx.z >= a.rows;
-  const int row = prefix ? ((int)blockIdx.z - a.rows) * a.group : (int)blockIdx.z;
+  const int kvh = blockIdx.x, slot = blockIdx.y, G = a.G;
+  const int row = prefix ? ((int)blockIdx.z - a.rows) * a.group : (int)blockIdx.z, chunk = prefix ? a.chunk_p : a.chunk;
   const int nq = prefix ? a.group * G : G;
   const int qi = col / CO::VAR, var = col % CO::VAR;
   const int my_row = prefix ? row + min(qi / G, a.group - 1) : row, my_head = kvh * G + (qi < nq ? qi % G : 0);
@@ -61,10 +66,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
   }
   const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
-  const int c0 = (prefix ? 0 : shared) + blockIdx.x * a.chunk;
+  if (slot >= (prefix ? a.slots_p : a.slots)) return;
+  const int c0 = (prefix ? 0 : shared) + slot * chunk;
   // page ids of this wave: page c0 + w + NW k in lane k; requested beside the lengths
   int ids = -1;
-  if (NW * lane + w < a.chunk && c0 + w + NW * lane < a.width) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
+  if (NW * lane + w < chunk && c0 + w + NW * lane < a.width) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
   const int my_len = min(max(a.lens[my_row], 0), a.width * KV4_PAGE);
   int top = my_len;                                                               // the longest of the rows here
   if (prefix) {
@@ -73,7 +79,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   }
   top = __builtin_amdgcn_readfirstlane(top);
   const int cols = (top + KV4_PAGE - 1) / KV4_PAGE;
-  const int c1 = min(c0 + a.chunk, prefix ? min(shared, cols) : cols);
+  const int c1 = min(c0 + chunk, prefix ? min(shared, cols) : cols);
   if (c0 >= c1 && a.ws) return;                                                   // nothing here (a row without tokens still gets its zeros)
   const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;                    // pages of this wave
   if (ids >= a.n_pages) ids = -1;
@@ -286,13 +292,12 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
     float L = 0.f, o = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      const float e = sm[i][qq] == -INFINITY && sl[i][qq] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sm[i][qq] - (M == -INFINITY ? 0.f : M));
+      const float e = __builtin_amdgcn_exp2f(sm[i][qq] - (M == -INFINITY ? 0.f : M));       // a wave without tokens: exp2(-infinity) = 0
       L = fmaf(sl[i][qq], e, L); o = fmaf(so[i][qq][d], e, o);
     }
     const int r = prefix ? row + qq / G : row, h = kvh * G + qq % G;
     if (a.ws) {
-      const int parts = a.group > 1 ? 2 : 1;                                      // prefix slots, then the row's own
-      float* p = a.ws + (((long)r * a.heads + h) * parts * a.slots + (prefix ? 0 : (parts - 1) * a.slots) + blockIdx.x) * (D + 2);
+      float* p = kv4_partial(a, D, r, h, (prefix ? 0 : a.slots_p) + slot);
       p[d] = o;
       if (d == 0) { p[D] = M; p[D + 1] = L; }
     } else {
@@ -301,52 +306,89 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   }
 }
 
-// the partials of a (row, head), in slot order
-template <int D>
-__global__ __launch_bounds__(D) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
-  const int len = min(max(a.lens[row], 0), a.width * KV4_PAGE), cols = (len + KV4_PAGE - 1) / KV4_PAGE;
-  const int parts = a.group > 1 ? 2 : 1;
-  int np = 0;
-  if (a.group > 1) {
-    int top = 0;                                                                  // a group's prefix workgroups go as far as its longest row
-    for (int j = 0; j < a.group; ++j) top = max(top, min(max(a.lens[row / a.group * a.group + j], 0), a.width * KV4_PAGE));
-    np = min(min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width), (top + KV4_PAGE - 1) / KV4_PAGE);
-  }
-  const int own = max(cols - (a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0), 0);
-  const float* base = a.ws + ((long)row * a.heads + h) * parts * a.slots * (D + 2);
-  const int n0 = (np + a.chunk - 1) / a.chunk, n1 = (own + a.chunk - 1) / a.chunk;
-  float M = -INFINITY;
-  for (int i = 0; i < n0 + n1; ++i) M = fmaxf(M, base[(long)(i < n0 ? i : (parts - 1) * a.slots + i - n0) * (D + 2) + D]);
-  float L = 0.f, o = 0.f;
-  for (int i = 0; i < n0 + n1; ++i) {
-    const float* p = base + (long)(i < n0 ? i : (parts - 1) * a.slots + i - n0) * (D + 2);
-    const float pm = p[D], pl = p[D + 1], e = pm == -INFINITY && pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(pm - (M == -INFINITY ? 0.f : M));
-    L = fmaf(pl, e, L); o = fmaf(p[d], e, o);
-  }
-  a.o[row * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : o / L);
+template <int D, int MODE, int NW, bool ALIBI>
+__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, ALIBI, false>(a); }
+
+// beam groups: z >= rows: a group's shared columns (up to 16 queries); below: a row's own
+template <int D, int MODE, bool ALIBI>
+__global__ __launch_bounds__(256) void kv4_attn_group_kernel(Kv4AttnArgs a) {
+  if ((int)blockIdx.z >= a.rows) kv4_attn_part<D, 2, 4, ALIBI, true>(a);
+  else kv4_attn_part<D, MODE, 4, ALIBI, false>(a);
 }
 
-struct Kv4Plan { int mode, nw, chunk, slots, group; int64_t floats; };
+// joins the partials of a (row, head): four groups of D threads, each an online pass over every fourth slot (all loads independent: one memory latency), then
+// the four in order
+#define KV4_MAX_SLOTS 256                                                         // of a row's own columns, and of its group's
+template <int D>
+__global__ __launch_bounds__(4 * D) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
+  __shared__ float so[4][D], sm[4], sl[4];
+  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D;
+  const int len = min(max(a.lens[row], 0), a.width * KV4_PAGE), cols = (len + KV4_PAGE - 1) / KV4_PAGE;
+  int np = 0, sh = 0;
+  if (a.slots_p) {
+    int top = 0;                                                                  // a group's workgroups go as far as its longest row
+    const int r0 = row / a.group * a.group;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, a.lens[r0 + min(j, a.group - 1)]);
+    top = min(top, a.width * KV4_PAGE);
+    sh = min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width);
+    np = min(sh, (top + KV4_PAGE - 1) / KV4_PAGE);
+  }
+  const int n0 = a.slots_p ? (np + a.chunk_p - 1) / a.chunk_p : 0, n = n0 + (max(cols - sh, 0) + a.chunk - 1) / a.chunk;
+  const float* base = kv4_partial(a, D, row, h, 0);
+  float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll 4
+  for (int i = part; i < n; i += 4) {
+    const float* p = base + (i < n0 ? i : a.slots_p + i - n0) * (D + 2);
+    const float pm = p[D], pl = p[D + 1], po = p[d], t = fmaxf(m, pm), u = t == -INFINITY ? 0.f : t;
+    const float r = __builtin_amdgcn_exp2f(m - u), e = __builtin_amdgcn_exp2f(pm - u);      // exp2(-infinity) = 0: nothing yet, or an empty partial
+    l = fmaf(pl, e, l * r); o = fmaf(po, e, o * r);
+    m = t;
+  }
+  so[part][d] = o;
+  if (d == 0) { sm[part] = m; sl[part] = l; }
+  __syncthreads();
+  if (part == 0) {
+    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), u = M == -INFINITY ? 0.f : M;
+    float L = 0.f, x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float e = __builtin_amdgcn_exp2f(sm[i] - u); L = fmaf(sl[i], e, L); x = fmaf(so[i][d], e, x); }
+    a.o[row * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : x / L);
+  }
+}
+
+struct Kv4Plan { int mode, nw, chunk, slots, group, chunk_p, slots_p; int64_t floats; };
 static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   Kv4Plan p;
-  const int G = d->heads / d->kv_heads, nbp = d->hd == 64 ? 2 : 4;
-  p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 ? d->group : 1;
-  const int nq = p.group > 1 ? p.group * G : G;                                   // one launch serves both kinds of workgroups
-  p.mode = nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : 2;
+  auto clamp = [](long x, long lo, long hi) { return (int)(x < lo ? lo : x > hi ? hi : x); };
+  auto mode = [&](int nq) { const int nbp = d->hd == 64 ? 2 : 4; return nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : 2; };
+  const int G = d->heads / d->kv_heads;
   const long units = (long)d->rows * d->kv_heads;
-  p.nw = p.mode < 2 && units < 512 ? 8 : 4;
-  const long want = (long)d->width * units / 1024;                                // pages of a workgroup that leave 1024 workgroups
-  p.chunk = (int)(want < 4 * p.nw ? 4 * p.nw : want > 32 * p.nw ? 32 * p.nw : want);
+  p.mode = mode(G);
+  p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 ? d->group : 1;
+  p.nw = p.mode == 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
+  p.chunk = clamp((long)d->width * units / 1024, units < 512 ? 4 * p.nw : 64, 64);
+  p.chunk_p = p.slots_p = 0;
+  if (p.group > 1) {
+    p.chunk = 64;
+    p.chunk_p = clamp((long)d->width * (units / p.group) / 512, 16, 64);
+    p.slots_p = (d->width + p.chunk_p - 1) / p.chunk_p;
+  }
+  // longer chunks where a row would have more partials than the merge is made for (over 524 288 tokens at 64 pages)
+  if (d->width > (long)KV4_MAX_SLOTS * p.chunk) p.chunk = (d->width + KV4_MAX_SLOTS - 1) / KV4_MAX_SLOTS;
+  if (p.group > 1 && d->width > (long)KV4_MAX_SLOTS * p.chunk_p) {
+    p.chunk_p = (d->width + KV4_MAX_SLOTS - 1) / KV4_MAX_SLOTS;
+    p.slots_p = (d->width + p.chunk_p - 1) / p.chunk_p;
+  }
   p.slots = d->width > 0 ? (d->width + p.chunk - 1) / p.chunk : 1;
-  p.floats = p.group == 1 && p.slots == 1 ? 0 : (int64_t)units * G * (p.group > 1 ? 2 : 1) * p.slots * (d->hd + 2);
+  p.floats = p.group == 1 && p.slots == 1 ? 0 : (int64_t)d->rows * d->heads * (p.slots + p.slots_p) * (d->hd + 2);
   return p;
 }
 static int kv4_attn_check(const unimp_kv4_attn_desc* d) {
   if (!d || !d->q || !d->pages || !d->tables || !d->lens || !d->out) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: null pointer");
-  if (d->kv_heads <= 0 || d->heads < 0 || d->heads % d->kv_heads || d->heads / d->kv_heads > 16 || d->width < 0 || d->width > (1 << 26) || d->rows < 0 || d->rows > 32767 ||
+  if (d->kv_heads <= 0 || d->heads < 0 || d->heads % d->kv_heads || d->heads / d->kv_heads > 16 || d->width < 0 || d->width > 64 * 4 * KV4_MAX_SLOTS || d->rows < 0 || d->rows > 32767 ||
       d->heads > 65535 || d->n_pages <= 0)
-    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 32767 rows, 2^26 pages of a row; a pool with pages");
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 32767 rows, 65536 pages of a row; a pool with pages");
   if (d->hd != 64 && d->hd != 80 && d->hd != 128) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
   if ((((uintptr_t)d->pages | (uintptr_t)d->q) & 15) || ((d->q_row_stride | d->q_head_stride) & 7))
     return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_attn_decode: 16-byte aligned pages and q, q strides multiples of 8 elements");
@@ -357,19 +399,37 @@ extern "C" int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc* d) { retu
 
 template <int D>
 static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
-  const dim3 grid(p.slots, a.kv_heads, a.rows + (p.group > 1 ? a.rows / p.group : 0));
+  if (p.group > 1) {
+    const dim3 grid(a.kv_heads, p.slots > p.slots_p ? p.slots : p.slots_p, a.rows + a.rows / p.group);
+#define KV4_G(M)                                                                                             \
+  do {                                                                                                       \
+    if (a.alibi) hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, true>), grid, dim3(256), 0, s, a);          \
+    else hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, false>), grid, dim3(256), 0, s, a);                 \
+  } while (0)
+    if (p.mode == 0) KV4_G(0);
+    else if (p.mode == 1) KV4_G(1);
+    else KV4_G(2);
+#undef KV4_G
+    hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(4 * D), 0, s, a);
+    return;
+  }
+  // key heads fastest: a row's chunks are of unequal use (the last ones mostly behind its end), and consecutive workgroups go to the eight dies in turn
+  const dim3 grid(a.kv_heads, p.slots, a.rows);
 #define KV4_L(M, W)                                                                                          \
   do {                                                                                                       \
     if (a.alibi) hipLaunchKernelGGL((kv4_attn_kernel<D, M, W, true>), grid, dim3(64 * W), 0, s, a);          \
     else hipLaunchKernelGGL((kv4_attn_kernel<D, M, W, false>), grid, dim3(64 * W), 0, s, a);                 \
   } while (0)
-  if (p.mode == 0 && p.nw == 8) KV4_L(0, 8);
-  else if (p.mode == 0) KV4_L(0, 4);
-  else if (p.mode == 1 && p.nw == 8) KV4_L(1, 8);
-  else if (p.mode == 1) KV4_L(1, 4);
+#define KV4_W(M)                                                                                             \
+  do {                                                                                                       \
+    if (p.nw == 8) KV4_L(M, 8); else if (p.nw == 4) KV4_L(M, 4); else KV4_L(M, 1); \
+  } while (0)
+  if (p.mode == 0) KV4_W(0);
+  else if (p.mode == 1) KV4_W(1);
   else KV4_L(2, 4);
+#undef KV4_W
 #undef KV4_L
-  if (a.ws) hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(D), 0, s, a);
+  if (a.ws) hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(4 * D), 0, s, a);
 }
 
 extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* workspace, void* stream) {
@@ -379,7 +439,7 @@ extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* worksp
   const Kv4Plan p = kv4_plan(d);
   if (p.floats && !workspace) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: workspace of unimp_kv4_attn_workspace floats");
   Kv4AttnArgs a{(const bf16*)d->q, d->q_row_stride, d->q_head_stride, (const uint8_t*)d->pages, d->n_pages, d->kv_heads, d->tables, d->table_stride, d->width, d->lens,
-                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, p.group, d->shared_len, d->heads / d->kv_heads, p.chunk, p.slots,
+                d->rows, d->heads, d->scale, d->alibi_slopes, (bf16*)d->out, d->o_row_stride, d->o_head_stride, p.group, d->shared_len, d->heads / d->kv_heads, p.chunk, p.slots, p.chunk_p, p.slots_p,
                 p.floats ? workspace : nullptr};
   switch (d->hd) {
     case 64: kv4_attn_launch<64>(a, p, (hipStream_t)stream); break;
