@@ -229,8 +229,10 @@ def test_reorder_beams(ops, K, groups, heads, hd, layers):
 @pytest.mark.parametrize("hd", [64, 80, 128])
 @pytest.mark.parametrize("rows,kvh,G,lens,alibi", [
     (1, 1, 1, [1], False), (5, 2, 1, [0, 1, 31, 32, 33], True), (3, 3, 2, [64, 7, 200], False), (2, 1, 16, [129, 300], True), (4, 2, 3, [96, 0, 1, 511], True),
-    (2, 4, 8, [1500, 40], False), (1, 2, 1, [4500], True)])
+    (2, 4, 8, [1500, 40], False), (1, 2, 1, [4500], True), (70, 16, 1, [5, 130, 64, 0, 513, 31, 200], False), (40, 32, 2, [77, 1, 90, 0], True),
+    (9, 2, 4, [3000, 0, 1777, 2111], True)])
 def test_attention(ops, hd, rows, kvh, G, lens, alibi):
+    lens = (lens * rows)[:rows]
     W = (max(lens) + 31) // 32 + 1
     pages, tables = paged(rows, W, kvh, hd, seed=rows + G)
     for r, n in enumerate(lens):                                    # tables name nothing valid behind a row's pages, and the last page's unused tokens hold garbage
@@ -267,7 +269,10 @@ def poison_behind(page, n, hd):
 
 
 @pytest.mark.parametrize("hd,K,groups,kvh,G,prompt,more", [(80, 10, 1, 4, 1, 100, 20), (128, 4, 2, 2, 2, 64, 70), (64, 5, 3, 1, 3, 31, 40), (80, 16, 1, 2, 1, 333, 1),
-                                                          (128, 10, 1, 2, 4, 200, 90), (64, 2, 2, 2, 8, 1000, 33)])
+                                                          (128, 10, 1, 2, 4, 200, 90), (64, 2, 2, 2, 8, 1000, 33),
+                                                          # from 8 192 pages of all rows and key heads on the shared pages are read once per group
+                                                          (80, 10, 2, 32, 1, 400, 20), (64, 16, 2, 32, 1, 290, 40), (128, 2, 5, 32, 8, 930, 70), (128, 4, 3, 32, 4, 700, 30),
+                                                          (80, 3, 2, 16, 2, 2700, 40), (64, 5, 2, 16, 3, 1663, 3)])
 def test_attention_beam_groups(ops, hd, K, groups, kvh, G, prompt, more):
     """the beams of a prompt name its whole pages together; with and without room for all their queries in one tile; ragged lengths behind the prompt"""
     rows = K * groups
@@ -343,6 +348,18 @@ def test_attention_not_a_number(ops):
     assert seen[0, 1].all() and seen[2, 1].all() and (~torch.isfinite(got[1, 0, 32:64])).all()
     nan[1, 0, 32:64] = True
     assert torch.isfinite(got[~nan]).all()
+
+
+def test_attention_wide_table(ops):
+    """a table far wider than its rows (the width is what the launch is made for, never the lengths), and one row of 20 000 tokens"""
+    hd, kvh, W = 64, 1, 40000
+    pages, few = paged(2, 640, kvh, hd, seed=61)
+    tables = torch.full((2, W), -1, dtype=torch.int32)
+    tables[:, :640] = few
+    lens = torch.tensor([20000, 45], dtype=torch.int32)
+    q = rnd(2, 2, hd, seed=62)
+    want, bound = R.attend(q, pages, tables[:, :640], lens, 0.125)
+    check(ops.kv4_attn_decode(q.cuda(), pages.cuda(), tables.cuda(), lens.cuda(), 0.125), want, bound)
 
 
 def test_hidden_pages(ops):

@@ -12,10 +12,12 @@
 //            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
 //            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 2: 16 queries, block and half as products.
 // Bound by the bytes of the pages: 17 / 32 of a byte per element.
+#include <type_traits>
 #include "kv4.h"
 #include "unimp_hip.h"
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
+#define KV4_TEAMS 4                    // rows of a workgroup on a beam group's tails
 
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
@@ -39,16 +41,25 @@ __device__ __forceinline__ float* kv4_partial(const Kv4AttnArgs& a, int D, int r
   return a.ws + (((long)row * a.heads + head) * (a.slots_p + a.slots) + slot) * (D + 2);
 }
 
-// prefix: the columns that a group's rows share, for the queries of all of them; else one row's own columns
-template <int D, int MODE, int NW, bool ALIBI, bool prefix>
+// prefix: the columns that a group's rows share, for the queries of all of them; else one row's own columns.  NW waves share the pages of a chunk; TEAMS > 1
+// (NW = 1): every wave of the workgroup has a row of its own.
+template <int D, int MODE, int NW, int TEAMS, bool ALIBI, bool prefix>
 __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   using P = Kv4<D>;
   using CO = Kv4Cols<D, MODE>;
   constexpr int NI = P::NI;
-  __shared__ float so[NW][CO::Q][D], sm[NW][CO::Q], sl[NW][CO::Q];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+  static_assert(TEAMS == 1 || NW == 1, "a team of several waves needs the workgroup's barrier");
+  __shared__ float team_o[TEAMS][NW][CO::Q][D], team_m[TEAMS][NW][CO::Q], team_l[TEAMS][NW][CO::Q];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int team = TEAMS > 1 ? wave : 0, w = TEAMS > 1 ? 0 : wave, tid = TEAMS > 1 ? lane : threadIdx.x;
+  float (&so)[NW][CO::Q][D] = team_o[team];
+  float (&sm)[NW][CO::Q] = team_m[team];
+  float (&sl)[NW][CO::Q] = team_l[team];
   const int kvh = blockIdx.x, slot = blockIdx.y, G = a.G;
-  const int row = prefix ? ((int)blockIdx.z - a.rows) * a.group : (int)blockIdx.z, chunk = prefix ? a.chunk_p : a.chunk;
+  const int row = prefix ? ((int)blockIdx.z - (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) * a.group : (int)blockIdx.z * TEAMS + team;
+  if (row >= a.rows) return;
+  const int chunk = prefix ? a.chunk_p : a.chunk, slots = prefix ? a.slots_p : a.slots;
+  if (slot >= slots) return;
   const int nq = prefix ? a.group * G : G;
   const int qi = col / CO::VAR, var = col % CO::VAR;
   const int my_row = prefix ? row + min(qi / G, a.group - 1) : row, my_head = kvh * G + (qi < nq ? qi % G : 0);
@@ -66,11 +77,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
     }
   }
   const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
-  if (slot >= (prefix ? a.slots_p : a.slots)) return;
-  const int c0 = (prefix ? 0 : shared) + slot * chunk;
-  // page ids of this wave: page c0 + w + NW k in lane k; requested beside the lengths
-  int ids = -1;
-  if (NW * lane + w < chunk && c0 + w + NW * lane < a.width) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane];
+  // page ids of this wave: page c0 + w + NW k in lane k; where one chunk holds the whole row they are requested beside the lengths
+  int ids = -1, c0 = prefix ? 0 : shared;
+  auto load_ids = [&](int pages) { if (NW * lane + w < pages && c0 + w + NW * lane < a.width) ids = a.tables[(long)row * a.t_stride + c0 + w + NW * lane]; };
+  if (slots == 1) load_ids(chunk);
   const int my_len = min(max(a.lens[my_row], 0), a.width * KV4_PAGE);
   int top = my_len;                                                               // the longest of the rows here
   if (prefix) {
@@ -79,13 +89,20 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   }
   top = __builtin_amdgcn_readfirstlane(top);
   const int cols = (top + KV4_PAGE - 1) / KV4_PAGE;
-  const int c1 = min(c0 + chunk, prefix ? min(shared, cols) : cols);
+  const int end = prefix ? min(shared, cols) : cols, nch = (max(end - c0, 0) + chunk - 1) / chunk;      // chunks in use
+  int c1 = min(c0 + chunk, end);
+  if (slots > 1) {                                                                // as many as there are, equally long
+    const int ch = nch > 0 ? (end - c0 + nch - 1) / nch : 0;
+    c0 += slot * ch;
+    c1 = min(c0 + ch, end);
+    load_ids(ch);
+  }
   if (c0 >= c1 && a.ws) return;                                                   // nothing here (a row without tokens still gets its zeros)
   const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;                    // pages of this wave
   if (ids >= a.n_pages) ids = -1;
 
   const uint32_t k_at = P::BLK_LAST < 32 && g == P::NB - 1 ? 512 * g + 8 * col : 512 * g + 16 * col, ks_at = P::KS + 32 * g + 2 * col;
-  const uint32_t v_at = P::VOFF + 4 * (g * D + col * NI), vs_at = P::VS + 8 * P::NB * g + (MODE == 2 ? 0 : 8 * min(MODE == 0 ? var >> 1 : var, P::NB - 1));
+  const uint32_t v_at = P::VOFF + 4 * (g * D + col * NI), vs_at = P::VS + 8 * P::NB * g + 8 * min(MODE == 0 ? var >> 1 : MODE == 1 ? var : col & 3, P::NB - 1);
   auto page_of = [&](int k) { return a.pages + ((long)max(__builtin_amdgcn_readlane(ids, k), 0) * a.kv_heads + kvh) * P::BYTES; };
   // every lane's loads of page k, unconditional (past the last page: that one again, from the cache), so that the number in flight is known everywhere
   auto load = [&](Kv4Frag<D>& f, int k) {
@@ -108,7 +125,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       f.v0 = *(const u32x4*)(page + v_at);
       if (D == 128) f.v1 = *(const u32x4*)(page + v_at + 16);
     }
-    if constexpr (MODE < 2) f.vs = *(const u32x2*)(page + vs_at);
+    f.vs = *(const u32x2*)(page + vs_at);                                        // of the lane's block; MODE 2: of block col & 3
   };
 
   Kv4Frag<D> fa, fb;
@@ -165,8 +182,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, qh, z, 4, 0, 0, ks, 0, sb);
       s[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ka, ql, z, 4, 0, 0, ks, 0, sb);
     }
-    uint32_t vs0, vs1;
-    if constexpr (MODE < 2) { vs0 = f.vs[0]; vs1 = f.vs[1]; }
+    uint32_t vs0 = f.vs[0], vs1 = f.vs[1];
     float x[8];
     const float at = ALIBI ? (float)(c * KV4_PAGE + 4 * g - my_len + 1) : 0.f;
 #pragma unroll
@@ -242,11 +258,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
     } else {
-      const uint8_t* sp = page_of(k) + vs_at;
-#pragma unroll
-      for (int blk = 0; blk < P::NB; ++blk) {
-        const u32x2 d = *(const u32x2*)(sp + 8 * blk);
-        uint32_t d0 = d[0], d1 = d[1];
+      auto block = [&](auto BLK) {                                                // four lanes hold the four blocks' scales: taken from the neighbour (quad_perm)
+        constexpr int blk = decltype(BLK)::value;
+        uint32_t d0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)vs0, blk * 0x55, 0xf, 0xf, true);
+        uint32_t d1 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)vs1, blk * 0x55, 0xf, 0xf, true);
         hide(d0, d1);
         B bh, bl;
 #pragma unroll
@@ -257,7 +272,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
         }
 #pragma unroll
         for (int i = 2 * blk; i < 2 * blk + 2; ++i) if (i < NI) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
-      }
+      };
+      block(std::integral_constant<int, 0>()); block(std::integral_constant<int, 1>());
+      if constexpr (P::NB > 2) block(std::integral_constant<int, 2>());
+      if constexpr (P::NB > 3) block(std::integral_constant<int, 3>());
     }
   };
 
@@ -283,7 +301,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
     if (mine && qi < nq) *(f32x4*)&so[w][qi][16 * i + 4 * g] = x;
   }
   if (var == 0 && g == 0) { sm[w][qi] = m; sl[w][qi] = l; }
-  __syncthreads();
+  if constexpr (TEAMS > 1) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else __syncthreads();
   for (int x = tid; x < nq * D; x += 64 * NW) {
     const int qq = x / D, d = x - qq * D;
     float M = sm[0][qq];
@@ -307,22 +328,22 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 }
 
 template <int D, int MODE, int NW, bool ALIBI>
-__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, ALIBI, false>(a); }
+__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
 
-// beam groups: z >= rows: a group's shared columns (up to 16 queries); below: a row's own
+// beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once
 template <int D, int MODE, bool ALIBI>
 __global__ __launch_bounds__(256) void kv4_attn_group_kernel(Kv4AttnArgs a) {
-  if ((int)blockIdx.z >= a.rows) kv4_attn_part<D, 2, 4, ALIBI, true>(a);
-  else kv4_attn_part<D, MODE, 4, ALIBI, false>(a);
+  if ((int)blockIdx.z >= (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) kv4_attn_part<D, 2, 4, 1, ALIBI, true>(a);
+  else kv4_attn_part<D, MODE, 1, KV4_TEAMS, ALIBI, false>(a);
 }
 
-// joins the partials of a (row, head): four groups of D threads, each an online pass over every fourth slot (all loads independent: one memory latency), then
-// the four in order
+// joins the partials of a (row, head): PARTS groups of threads, two dims to a thread, each an online pass over every PARTS-th slot (all loads independent: one
+// memory latency), then the groups in order
 #define KV4_MAX_SLOTS 256                                                         // of a row's own columns, and of its group's
-template <int D>
-__global__ __launch_bounds__(4 * D) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
-  __shared__ float so[4][D], sm[4], sl[4];
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D;
+template <int D, int PARTS>
+__global__ __launch_bounds__(PARTS * D / 2) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
+  __shared__ float so[PARTS][D], sm[PARTS], sl[PARTS];
+  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x % (D / 2) * 2, part = threadIdx.x / (D / 2);
   const int len = min(max(a.lens[row], 0), a.width * KV4_PAGE), cols = (len + KV4_PAGE - 1) / KV4_PAGE;
   int np = 0, sh = 0;
   if (a.slots_p) {
@@ -334,27 +355,35 @@ __global__ __launch_bounds__(4 * D) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
     sh = min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width);
     np = min(sh, (top + KV4_PAGE - 1) / KV4_PAGE);
   }
-  const int n0 = a.slots_p ? (np + a.chunk_p - 1) / a.chunk_p : 0, n = n0 + (max(cols - sh, 0) + a.chunk - 1) / a.chunk;
+  // chunks in use, as kv4_attn_part counts them: ceil(columns / chunk) of equal length, so the last of them may have none left
+  auto used = [](int columns, int chunk) { const int k = (columns + chunk - 1) / chunk, ch = k > 0 ? (columns + k - 1) / k : 1; return (columns + ch - 1) / ch; };
+  const int n0 = a.slots_p ? used(np, a.slots_p > 1 ? a.chunk_p : max(np, 1)) : 0, own = max(cols - sh, 0), n = n0 + used(own, a.slots > 1 ? a.chunk : max(own, 1));
   const float* base = kv4_partial(a, D, row, h, 0);
-  float m = -INFINITY, l = 0.f, o = 0.f;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll 4
-  for (int i = part; i < n; i += 4) {
+  for (int i = part; i < n; i += PARTS) {
     const float* p = base + (i < n0 ? i : a.slots_p + i - n0) * (D + 2);
-    const float pm = p[D], pl = p[D + 1], po = p[d], t = fmaxf(m, pm), u = t == -INFINITY ? 0.f : t;
-    const float r = __builtin_amdgcn_exp2f(m - u), e = __builtin_amdgcn_exp2f(pm - u);      // exp2(-infinity) = 0: nothing yet, or an empty partial
-    l = fmaf(pl, e, l * r); o = fmaf(po, e, o * r);
+    const float2 st = *(const float2*)(p + D), po = *(const float2*)(p + d);
+    const float t = fmaxf(m, st.x), u = t == -INFINITY ? 0.f : t;
+    const float r = __builtin_amdgcn_exp2f(m - u), e = __builtin_amdgcn_exp2f(st.x - u);    // exp2(-infinity) = 0: nothing yet, or an empty partial
+    l = fmaf(st.y, e, l * r); o0 = fmaf(po.x, e, o0 * r); o1 = fmaf(po.y, e, o1 * r);
     m = t;
   }
-  so[part][d] = o;
-  if (d == 0) { sm[part] = m; sl[part] = l; }
-  __syncthreads();
-  if (part == 0) {
-    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), u = M == -INFINITY ? 0.f : M;
-    float L = 0.f, x = 0.f;
+  if constexpr (PARTS > 1) {
+    so[part][d] = o0; so[part][d + 1] = o1;
+    if (d == 0) { sm[part] = m; sl[part] = l; }
+    __syncthreads();
+    if (part) return;
+    m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { const float e = __builtin_amdgcn_exp2f(sm[i] - u); L = fmaf(sl[i], e, L); x = fmaf(so[i][d], e, x); }
-    a.o[row * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : x / L);
+    for (int i = 0; i < PARTS; ++i) m = fmaxf(m, sm[i]);
+    const float u = m == -INFINITY ? 0.f : m;
+    l = o0 = o1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) { const float e = __builtin_amdgcn_exp2f(sm[i] - u); l = fmaf(sl[i], e, l); o0 = fmaf(so[i][d], e, o0); o1 = fmaf(so[i][d + 1], e, o1); }
   }
+  bf16* o = a.o + row * a.o_rs + h * a.o_hs + d;
+  o[0] = f2bf(l == 0.f ? 0.f : o0 / l); o[1] = f2bf(l == 0.f ? 0.f : o1 / l);
 }
 
 struct Kv4Plan { int mode, nw, chunk, slots, group, chunk_p, slots_p; int64_t floats; };
@@ -365,12 +394,14 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   const int G = d->heads / d->kv_heads;
   const long units = (long)d->rows * d->kv_heads;
   p.mode = mode(G);
-  p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 ? d->group : 1;
+  // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads, pages = rows x heads x columns: 10 beams x 80, prompt
+  // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
+  p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
   p.nw = p.mode == 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
   p.chunk = clamp((long)d->width * units / 1024, units < 512 ? 4 * p.nw : 64, 64);
   p.chunk_p = p.slots_p = 0;
   if (p.group > 1) {
-    p.chunk = 64;
+    p.chunk = 16;
     p.chunk_p = clamp((long)d->width * (units / p.group) / 512, 16, 64);
     p.slots_p = (d->width + p.chunk_p - 1) / p.chunk_p;
   }
@@ -398,9 +429,15 @@ static int kv4_attn_check(const unimp_kv4_attn_desc* d) {
 extern "C" int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc* d) { return kv4_attn_check(d) || !d->rows || !d->heads ? 0 : kv4_plan(d).floats; }
 
 template <int D>
+static void kv4_merge_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
+  const dim3 grid(a.heads, a.rows);
+  if (p.slots + p.slots_p <= 8) hipLaunchKernelGGL((kv4_attn_merge_kernel<D, 1>), grid, dim3(D / 2), 0, s, a);
+  else hipLaunchKernelGGL((kv4_attn_merge_kernel<D, 8>), grid, dim3(4 * D), 0, s, a);
+}
+template <int D>
 static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
   if (p.group > 1) {
-    const dim3 grid(a.kv_heads, p.slots > p.slots_p ? p.slots : p.slots_p, a.rows + a.rows / p.group);
+    const dim3 grid(a.kv_heads, p.slots > p.slots_p ? p.slots : p.slots_p, (a.rows + KV4_TEAMS - 1) / KV4_TEAMS + a.rows / p.group);
 #define KV4_G(M)                                                                                             \
   do {                                                                                                       \
     if (a.alibi) hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, true>), grid, dim3(256), 0, s, a);          \
@@ -410,7 +447,7 @@ static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t 
     else if (p.mode == 1) KV4_G(1);
     else KV4_G(2);
 #undef KV4_G
-    hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(4 * D), 0, s, a);
+    kv4_merge_launch<D>(a, p, s);
     return;
   }
   // key heads fastest: a row's chunks are of unequal use (the last ones mostly behind its end), and consecutive workgroups go to the eight dies in turn
@@ -429,7 +466,7 @@ static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t 
   else KV4_L(2, 4);
 #undef KV4_W
 #undef KV4_L
-  if (a.ws) hipLaunchKernelGGL((kv4_attn_merge_kernel<D>), dim3(a.heads, a.rows), dim3(4 * D), 0, s, a);
+  if (a.ws) kv4_merge_launch<D>(a, p, s);
 }
 
 extern "C" int unimp_kv4_attn_decode(const unimp_kv4_attn_desc* d, float* workspace, void* stream) {
