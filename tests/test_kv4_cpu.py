@@ -56,7 +56,7 @@ def test_python_refusals():
     _bad("heads", lambda: ops.kv4_write(k, k, _pool(heads=3), s3))
     _bad("page bytes of another head dim", lambda: ops.kv4_write(k, k, _pool(hd=80), s3))
     _bad("k and v differ", lambda: ops.kv4_write(k, k[:2], _pool(), s3))
-    _bad("fp16", lambda: (ops._kv4_rows(k.half(), 64)))
+    _bad("fp16", lambda: ops.kv4_write(k.half(), k.half(), _pool(), s3))
     _bad("int32 slots", lambda: ops.kv4_write(k, k, _pool(), s3.int()))
     _bad("strided slots", lambda: ops.kv4_write(k, k, _pool(), torch.zeros(6, dtype=i64)[::2]))
     _bad("pages not contiguous", lambda: ops.kv4_write(k, k, _pool(heads=4)[:, ::2], s3))
@@ -121,3 +121,13 @@ def test_c_refusals():
     assert at(q=None) == at(lens=None) == at(out=None) == ARG and at(heads=5) == at(heads=34) == at(hd=32) == at(kv_heads=0) == at(rows=1 << 17) == at(width=-1) == SHAPE
     assert at(pages=odd) == ALIGN and at(rows=0) == 0
     assert L.unimp_struct_size(5) == C.sizeof(_lib.Kv4AttnDesc)
+
+
+def test_packed_descriptor_is_the_struct():
+    """the wrapper packs the descriptor by a format string: the same bytes as the ctypes mirror's"""
+    vals = [11, 12, 13, 14, 15, 16, 17, 18, 19, 20, 21, 22, 23, 0.375, 24, 25, 26, 27, 28, 29]
+    d = _lib.Kv4AttnDesc(*vals)
+    packed = ops._KV4_ATTN.pack(*vals)
+    assert len(packed) == C.sizeof(d) or len(packed) == C.sizeof(d) - C.sizeof(d) % 8
+    again = _lib.Kv4AttnDesc.from_buffer_copy(packed.ljust(C.sizeof(d), b"\0"))
+    assert [getattr(again, n) for n, _ in d._fields_] == vals

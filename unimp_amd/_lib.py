@@ -119,7 +119,7 @@ _SIGS = {
     "unimp_page_tables_extend": [c_p, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_p, c_p, c_p, c_l, c_p, c_p],
     "unimp_kv4_reorder_beams": [c_p, c_l, c_i, c_l, c_i, c_i, c_p, c_i, c_i, c_i, c_p, c_p, c_p],
     "unimp_kv4_attn_workspace": [C.POINTER(Kv4AttnDesc)],
-    "unimp_kv4_attn_decode": [C.POINTER(Kv4AttnDesc), c_p, c_p],
+    "unimp_kv4_attn_decode": [c_p, c_p, c_p],          # a packed Kv4AttnDesc (ops._KV4_ATTN) or a pointer to one
     "unimp_image_resize_normalize": [c_p, c_p, c_i, c_i, c_p, c_p, c_i, c_i, c_p, c_p, c_p, c_i, c_p, c_p],
 }
 

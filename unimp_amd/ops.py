@@ -3,8 +3,10 @@
 Every tensor must live on a HIP device; nothing here has a CPU or eager-PyTorch fallback.
 """
 import ctypes as C
+import functools
 import json
 import os
+import struct
 import torch
 
 from . import _lib
@@ -1072,89 +1074,99 @@ def gemm_mx(a, b, *, bias=None, act=None, pre=None, aux=None, res=None, out=None
 
 
 # ----------------------------------------------------------------------------------------------- paged K/V cache held in 4 bits (decode)
+# These are called once per layer and token: the host's share of a small call is its time, so every wrapper checks its arguments in one expression and explains
+# (_kv4_refuse) only a call that fails it.
 KV4_PAGE = 32                                                 # tokens of a page
+_KV4_BYTES = {64: 2176, 80: 2752, 128: 4352}                  # head dim -> bytes of a page
+_KV4_HD = {b: h for h, b in _KV4_BYTES.items()}
+_i32, _i64, _u8, _f32 = torch.int32, torch.int64, torch.uint8, torch.float32
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def kv4_page_bytes(hd):
     """bytes of one page (32 tokens of one head of one layer, keys and values) at head dim 64, 80 or 128"""
-    if hd not in (64, 80, 128):
+    if hd not in _KV4_BYTES:
         raise ValueError(f"the 4-bit cache serves head dims 64, 80 and 128, not {hd}")
-    return 32 * hd + 64 * ((hd + 31) // 32)
+    return _KV4_BYTES[hd]
 
 
-def _same_device(*ts):
-    """every given tensor on one HIP device, and that device current: a launch goes to the current device's stream"""
-    dev = _dev(ts[0]).device
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise _lib.UnimpHipError(f"tensors on {dev} and {t.device}")
-    if dev.index != torch.cuda.current_device():
-        raise _lib.UnimpHipError(f"tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+def _kv4_refuse(what, rule, **args):
+    """the error of a call that its wrapper refuses"""
+    say = lambda t: f"{str(t.dtype)[6:]}{list(t.shape)} strides {list(t.stride())} on {t.device}" if torch.is_tensor(t) else repr(t)
+    raise ValueError(f"{what}: {rule}; got " + ", ".join(f"{k} = {say(v)}" for k, v in args.items()))
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _kv4_launch(fn, what, tensors, args):
+    """the launch on the current stream, if every tensor lives on the current HIP device (its stream would not order the call otherwise)"""
+    dev = _current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise _lib.UnimpHipError(f"{what}: every tensor on the current HIP device ({'none' if dev < 0 else f'cuda:{dev}'}), got {t.device}")
+    rc = fn(*args, _raw_stream(dev) if _raw_stream is not None else _stream())
+    if rc:
+        check(rc, what)
 
 
-def _kv4_pool(pages, hd, layered=False):
-    """checks a pool [(layers,) n_pages, heads, page bytes] -> (layers, byte stride between layers, n_pages, heads)"""
-    pb = kv4_page_bytes(hd)
-    _need(pages.dtype == torch.uint8 and pages.dim() in ((3, 4) if layered else (3,)) and pages.shape[-1] == pb and pages.stride()[-3:] == (pages.shape[-2] * pb, pb, 1),
-          f"pages: uint8 [{'layers, ' if layered else ''}n_pages, heads, {pb}] for head dim {hd}, a layer's pages contiguous; got {tuple(pages.shape)} {pages.dtype}")
-    layers, stride = (pages.shape[0], pages.stride(0)) if pages.dim() == 4 else (1, 0)
-    _need(layers == 1 or stride >= pages.shape[-3] * pages.shape[-2] * pb, "pages: layers overlap")
-    return layers, stride, pages.shape[-3], pages.shape[-2]
-
-
-def _kv4_rows(t, hd):
+def _kv4_rows(t):
     """a [tokens, heads, hd] bf16 view whose 8-element pieces are 16-byte aligned (copied only if it is not one)"""
-    _need(t.dtype == bf16 and t.dim() == 3 and t.shape[2] == hd, f"expected bf16 [tokens, heads, {hd}], got {t.dtype} {tuple(t.shape)}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-    return t
+    st = t.stride()
+    return t if st[2] == 1 and not (st[0] & 7 or st[1] & 7 or t.data_ptr() & 15) else t.contiguous()
 
 
 def kv4_write(k, v, pages, slots):
     """quantise k and v [tokens, heads, hd] (bf16 views, e.g. a prefill's rotated keys) into the slots [tokens] (int64; slot s = token s % 32 of page s // 32; a slot
     outside the pool: the token is not written) of one layer's pages [n_pages, heads, kv4_page_bytes(hd)]."""
-    hd = k.shape[-1]
-    _, _, n_pages, heads = _kv4_pool(pages, hd)
-    _need(k.shape == v.shape and k.shape[1] == heads, f"k {tuple(k.shape)}, v {tuple(v.shape)}: [tokens, {heads}, {hd}]")
-    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.numel() == k.shape[0] and slots.is_contiguous(), "slots: contiguous int64 [tokens]")
-    _same_device(pages, k, v, slots)
-    k, v = _kv4_rows(k, hd), _kv4_rows(v, hd)
-    check(_lib.lib().unimp_kv4_write(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), pages.data_ptr(), n_pages, heads, hd,
-                                      slots.data_ptr(), k.shape[0], _stream()), "kv4_write")
+    if not (k.dim() == 3 and k.shape == v.shape and k.dtype is bf16 and v.dtype is bf16 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous()
+            and pages.shape[2] == _KV4_BYTES.get(k.shape[2]) and pages.shape[1] == k.shape[1] and slots.dtype is _i64 and slots.dim() == 1
+            and slots.shape[0] == k.shape[0] and slots.is_contiguous()):
+        _kv4_refuse("kv4_write", "k, v bf16 [tokens, heads, hd]; pages contiguous uint8 [n_pages, heads, kv4_page_bytes(hd)]; slots contiguous int64 [tokens]", k=k, v=v, pages=pages,
+                    slots=slots)
+    k, v = _kv4_rows(k), _kv4_rows(v)
+    (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+    _kv4_launch(_lib.lib().unimp_kv4_write, "kv4_write", (pages, k, v, slots), (k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, pages.data_ptr(), pages.shape[0], k.shape[1],
+                                                                                k.shape[2], slots.data_ptr(), k.shape[0]))
 
 
 def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows, pages, slots):
     """decode step on the 4-bit cache: rotate q and k of every row (row r with ITS table row cos_rows / sin_rows [rows, rot // 2]; rot = 0: none), quantise the
     rotated k and v into slot slots[r] of one layer's pages, return the rotated q [rows, heads, hd].  Operand layout of decode_rope_append; qkv2d is left unrotated."""
-    _, _, n_pages, ph = _kv4_pool(pages, hd)
-    rows = qkv2d.shape[0]
-    _need(qkv2d.dtype == bf16 and qkv2d.dim() == 2 and qkv2d.stride(1) == 1 and ph == heads, f"qkv: bf16 rows with unit stride, {ph} heads")
-    _need(len(offs) == 3 and min(offs) >= 0 and head_stride >= 0 and max(offs) + (heads - 1) * head_stride + hd <= qkv2d.shape[1], "q / k / v offsets outside the row")
-    _need(0 <= rot <= hd and rot % 2 == 0, f"rot {rot}: even, at most the head dim")
-    _need(slots.dtype == torch.int64 and slots.shape == (rows,) and slots.is_contiguous(), "slots: contiguous int64 [rows]")
-    if rot:
-        _need(all(t.dtype == torch.float32 and t.shape == (rows, rot // 2) and t.is_contiguous() for t in (cos_rows, sin_rows)), "cos / sin: contiguous fp32 [rows, rot // 2]")
-    _same_device(pages, qkv2d, slots, cos_rows if rot else None, sin_rows if rot else None)
-    q = torch.empty((rows, heads, hd), dtype=bf16, device=qkv2d.device)
-    check(_lib.lib().unimp_kv4_rope_append(qkv2d.data_ptr(), qkv2d.stride(0), head_stride, rows, heads, hd, offs[0], offs[1], offs[2], rot, _p(cos_rows) if rot else 0,
-                                            _p(sin_rows) if rot else 0, q.data_ptr(), pages.data_ptr(), n_pages, slots.data_ptr(), _stream()), "kv4_rope_append")
+    rows, width = qkv2d.shape
+    q_off, k_off, v_off = offs
+    if not (qkv2d.dtype is bf16 and qkv2d.stride(1) == 1 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous() and pages.shape[1] == heads
+            and pages.shape[2] == _KV4_BYTES.get(hd) and min(q_off, k_off, v_off, head_stride) >= 0 and max(q_off, k_off, v_off) + (heads - 1) * head_stride + hd <= width
+            and slots.dtype is _i64 and slots.shape == (rows,) and slots.is_contiguous()
+            and (rot == 0 or (0 < rot <= hd and not rot & 1 and cos_rows.dtype is _f32 and sin_rows.dtype is _f32 and cos_rows.shape == (rows, rot // 2) == sin_rows.shape
+                              and cos_rows.is_contiguous() and sin_rows.is_contiguous()))):
+        _kv4_refuse("kv4_rope_append", "qkv bf16 rows with q, k, v of every head inside; pages contiguous uint8 [n_pages, heads, kv4_page_bytes(hd)]; slots contiguous int64 [rows]; "
+                    "rot even, at most hd; cos, sin contiguous fp32 [rows, rot // 2]", qkv=qkv2d, heads=heads, head_stride=head_stride, hd=hd, offs=offs, rot=rot, cos=cos_rows,
+                    sin=sin_rows, pages=pages, slots=slots)
+    q = qkv2d.new_empty((rows, heads, hd))
+    _kv4_launch(_lib.lib().unimp_kv4_rope_append, "kv4_rope_append", (pages, qkv2d, slots) + ((cos_rows, sin_rows) if rot else ()),
+                (qkv2d.data_ptr(), qkv2d.stride(0), head_stride, rows, heads, hd, q_off, k_off, v_off, rot, cos_rows.data_ptr() if rot else None,
+                 sin_rows.data_ptr() if rot else None, q.data_ptr(), pages.data_ptr(), pages.shape[0], slots.data_ptr()))
     return q
+
+
+def _kv4_layers(pages):
+    """(layers, bytes between them) of a pool [(layers,) n_pages, heads, page bytes] of uint8 whose layers are contiguous; layers 0: it is not one"""
+    sh, st = pages.shape, pages.stride()
+    if pages.dtype is not _u8 or not 3 <= len(sh) <= 4 or st[-3:] != (sh[-2] * sh[-1], sh[-1], 1):
+        return 0, 0
+    if len(sh) == 3:
+        return 1, 0
+    return (sh[0], st[0]) if sh[0] == 1 or st[0] >= sh[1] * sh[2] * sh[3] else (0, 0)
 
 
 def kv4_read(pages, slots, hd):
     """the values held in slots [tokens] (int64; outside the pool: zeros) of pages [(layers,) n_pages, heads, kv4_page_bytes(hd)] -> k, v bf16
     [(layers,) tokens, heads, hd]: exactly what the attention multiplies"""
-    layers, stride, n_pages, heads = _kv4_pool(pages, hd, layered=True)
-    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.is_contiguous(), "slots: contiguous int64 [tokens]")
-    _same_device(pages, slots)
-    shape = tuple(pages.shape[:-3]) + (slots.numel(), heads, hd)
+    layers, stride = _kv4_layers(pages)
+    if not (layers and pages.shape[-1] == _KV4_BYTES.get(hd) and slots.dtype is _i64 and slots.dim() == 1 and slots.is_contiguous()):
+        _kv4_refuse("kv4_read", "pages uint8 [(layers,) n_pages, heads, kv4_page_bytes(hd)], every layer contiguous; slots contiguous int64 [tokens]", pages=pages, slots=slots, hd=hd)
+    tokens, (n_pages, heads) = slots.shape[0], pages.shape[-3:-1]
+    shape = (*pages.shape[:-3], tokens, heads, hd)
     k, v = torch.empty(shape, dtype=bf16, device=pages.device), torch.empty(shape, dtype=bf16, device=pages.device)
-    check(_lib.lib().unimp_kv4_read(pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), slots.numel(), k.data_ptr(), v.data_ptr(), _stream()), "kv4_read")
+    _kv4_launch(_lib.lib().unimp_kv4_read, "kv4_read", (pages, slots), (pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr()))
     return k, v
 
 
@@ -1165,19 +1177,23 @@ def page_tables_extend(tables, mapped, cached, new, free_pages, cursor, max_toke
     [rows // group]): the rows of a group take their first row's pages below shared_len // 32 columns.
     Returns (mapped, cursor, slots, cu): the new column counts and free-list position (above n: pages were missing, their columns are -1), slots int64 [max_tokens] of
     the new tokens in packed order (-1: none) and int32 [rows + 1] the packed index of every row's first new token."""
-    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous() and tables.numel() > 0, "tables: contiguous int32 [rows, width]")
     rows, width = tables.shape
-    for name, t, n in (("mapped", mapped, rows), ("cached", cached, rows), ("new", new, rows), ("cover", cover, rows), ("cursor", cursor, 1),
-                       ("shared_len", shared_len, rows // max(group, 1))):
-        _need(t is None or (t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()), f"{name}: contiguous int32 [{n}]")
-    _need(free_pages.dtype == torch.int32 and free_pages.dim() == 1 and free_pages.is_contiguous() and free_pages.numel() < 2 ** 31, "free_pages: contiguous int32 [n]")
-    _need(group >= 1 and rows % group == 0 and max_tokens >= 0, f"{rows} rows in groups of {group}, room for {max_tokens} tokens")
-    _same_device(tables, mapped, cached, new, free_pages, cursor, cover, shared_len)
-    i32 = lambda n: torch.empty(n, dtype=torch.int32, device=tables.device)
-    mapped_out, cursor_out, cu, slots = i32(rows), i32(1), i32(rows + 1), torch.empty(max_tokens, dtype=torch.int64, device=tables.device)
-    check(_lib.lib().unimp_page_tables_extend(tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), _p(cover), free_pages.data_ptr(),
-                                               free_pages.numel(), cursor.data_ptr(), group, _p(shared_len), mapped_out.data_ptr(), cursor_out.data_ptr(),
-                                               slots.data_ptr(), max_tokens, cu.data_ptr(), _stream()), "page_tables_extend")
+    if not (tables.dtype is _i32 and tables.is_contiguous() and rows * width > 0 and group >= 1 and rows % group == 0 and max_tokens >= 0
+            and mapped.dtype is _i32 and mapped.shape == (rows,) and mapped.is_contiguous() and cached.dtype is _i32 and cached.shape == (rows,) and cached.is_contiguous()
+            and new.dtype is _i32 and new.shape == (rows,) and new.is_contiguous() and cursor.dtype is _i32 and cursor.shape == (1,)
+            and free_pages.dtype is _i32 and free_pages.dim() == 1 and free_pages.is_contiguous()
+            and (cover is None or (cover.dtype is _i32 and cover.shape == (rows,) and cover.is_contiguous()))
+            and (shared_len is None or (shared_len.dtype is _i32 and shared_len.shape == (rows // group,) and shared_len.is_contiguous()))):
+        _kv4_refuse("page_tables_extend", "contiguous int32: tables [rows, width], mapped, cached, new, cover [rows], free_pages [n], cursor [1], shared_len [rows // group]; rows a multiple "
+                    "of group", tables=tables, mapped=mapped, cached=cached, new=new, cover=cover, free_pages=free_pages, cursor=cursor, group=group, shared_len=shared_len,
+                    max_tokens=max_tokens)
+    dev = tables.device
+    ints, slots = torch.empty(2 * rows + 2, dtype=_i32, device=dev), torch.empty(max_tokens, dtype=_i64, device=dev)
+    p = ints.data_ptr()                                       # mapped [rows], cursor [1], cu [rows + 1]
+    _kv4_launch(_lib.lib().unimp_page_tables_extend, "page_tables_extend", (tables, mapped, cached, new, free_pages, cursor, cover, shared_len),
+                (tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), None if cover is None else cover.data_ptr(), free_pages.data_ptr(),
+                 free_pages.shape[0], cursor.data_ptr(), group, None if shared_len is None else shared_len.data_ptr(), p, p + 4 * rows, slots.data_ptr(), max_tokens, p + 4 * rows + 4))
+    mapped_out, cursor_out, cu = ints.split((rows, 1, rows + 1))
     return mapped_out, cursor_out, slots, cu
 
 
@@ -1185,52 +1201,56 @@ def kv4_reorder_beams(pages, tables, group, src_local, pos):
     """beam search on the 4-bit cache, in place, all layers in one launch: row j of every group goes on with the hypothesis of row src_local[g * group + j] (int64, index
     inside the group); pos int64 [rows] = tokens cached (the same in a group).  Full pages change hands in tables [rows, width] (int32), the page that is being
     filled is copied in pages [(layers,) n_pages, heads, page bytes] into the row's own."""
-    hd = _kv4_hd(pages)
-    layers, stride, n_pages, heads = _kv4_pool(pages, hd, layered=True)
-    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous() and group >= 1 and tables.shape[0] % group == 0, "tables: contiguous int32 [rows, width]")
-    _need(all(t.dtype == torch.int64 and t.shape == (tables.shape[0],) and t.is_contiguous() for t in (src_local, pos)), "src_local, pos: contiguous int64 [rows]")
-    _same_device(pages, tables, src_local, pos)
-    check(_lib.lib().unimp_kv4_reorder_beams(pages.data_ptr(), stride, layers, n_pages, heads, hd, tables.data_ptr(), tables.shape[1], group, tables.shape[0] // group,
-                                              src_local.data_ptr(), pos.data_ptr(), _stream()), "kv4_reorder_beams")
+    layers, stride = _kv4_layers(pages)
+    rows, width = tables.shape
+    hd = _KV4_HD.get(pages.shape[-1], 0)
+    if not (layers and hd and tables.dtype is _i32 and tables.is_contiguous() and 1 <= group <= 16 and rows % group == 0 and src_local.dtype is _i64 and pos.dtype is _i64
+            and src_local.shape == (rows,) == pos.shape and src_local.is_contiguous() and pos.is_contiguous()):
+        _kv4_refuse("kv4_reorder_beams", "pages uint8 [(layers,) n_pages, heads, page bytes], every layer contiguous; tables contiguous int32 [rows, width], rows a multiple of group (at most "
+                    "16); src_local, pos contiguous int64 [rows]", pages=pages, tables=tables, group=group, src_local=src_local, pos=pos)
+    _kv4_launch(_lib.lib().unimp_kv4_reorder_beams, "kv4_reorder_beams", (pages, tables, src_local, pos),
+                (pages.data_ptr(), stride, layers, pages.shape[-3], pages.shape[-2], hd, tables.data_ptr(), width, group, rows // group, src_local.data_ptr(), pos.data_ptr()))
 
 
-def _kv4_hd(pages):
-    for hd in (64, 80, 128):
-        if pages.shape[-1] == kv4_page_bytes(hd):
-            return hd
-    raise ValueError(f"pages of {pages.shape[-1]} bytes: {[kv4_page_bytes(h) for h in (64, 80, 128)]} are those of head dims 64, 80 and 128")
+_KV4_ATTN = struct.Struct("@PqqPqiiPqiPiifPPqqiP")              # unimp_kv4_attn_desc (tests/test_kv4_cpu.py compares it with the ctypes mirror)
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace(rows, heads, kv_heads, hd, width, group):
+    """floats of the partials that a call of these sizes writes (0: none)"""
+    d = _lib.Kv4AttnDesc()
+    d.q = d.pages = d.tables = d.lens = d.out = d.shared_len = 1 << 20                # never followed
+    d.n_pages, d.kv_heads, d.hd, d.width, d.rows, d.heads, d.group = 1, kv_heads, hd, width, rows, heads, group
+    if group == 1:
+        d.shared_len = None
+    return int(_lib.lib().unimp_kv4_attn_workspace(C.byref(d)))
 
 
 def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_len=None, out=None):
     """attention of one new token per row over the 4-bit cache: q [rows, heads, hd] (bf16 view) against the first lens[r] (int32 [rows]) tokens of the pages that
-    tables [rows, width] (int32) name in one layer's pool [n_pages, kv heads, page bytes]; heads a multiple of kv heads.  alibi: fp32 [heads] slopes.  A row of length 0
-    gives zeros; a page id outside the pool hides its tokens.  group > 1 with shared_len (int32 [rows // group]): the rows of a group (the beams of a prompt) name the
-    same pages below shared_len // 32 columns; those are read once per group.  Returns o [rows, heads, hd]."""
-    _need(q.dim() == 3 and q.dtype == bf16 and q.stride(2) == 1, "q: bf16 [rows, heads, hd] with unit dim stride")
-    rows, heads, hd = q.shape
-    _, _, n_pages, kv_heads = _kv4_pool(pages, hd)
-    _need(kv_heads > 0 and heads % kv_heads == 0 and heads // kv_heads <= 16, f"{heads} query heads on {kv_heads} key heads: a multiple, at most 16 to one")
-    _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == rows and (tables.stride(1) == 1 or tables.shape[1] <= 1), "tables: int32 [rows, width], unit column stride")
-    _need(lens.dtype == torch.int32 and lens.shape == (rows,) and lens.is_contiguous(), "lens: contiguous int32 [rows]")
-    if alibi is not None:
-        _need(alibi.dtype == torch.float32 and alibi.numel() == heads and alibi.is_contiguous(), "alibi: contiguous fp32 [heads]")
-    if shared_len is not None:
-        _need(group >= 1 and rows % group == 0 and shared_len.dtype == torch.int32 and shared_len.numel() == rows // group and shared_len.is_contiguous(),
-              "shared_len: contiguous int32 [rows // group]")
+    tables [rows, width] (int32) name in one layer's pool [n_pages, kv heads, page bytes]; heads a multiple of kv heads, at most 16 to one.  alibi: fp32 [heads] slopes.  A
+    row of length 0 gives zeros; a page id outside the pool hides its tokens.  group > 1 with shared_len (int32 [rows // group]): the rows of a group (the beams of a
+    prompt) name the same pages below shared_len // 32 columns; those are read once per group.  Returns o [rows, heads, hd]."""
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=bf16, device=q.device)
-    _need(out.dtype == bf16 and out.shape == q.shape and out.stride(2) == 1, "out: bf16 like q, unit dim stride")
-    _same_device(pages, q, tables, lens, alibi, shared_len, out)
-    q = _kv4_rows(q, hd)
-    d = _lib.Kv4AttnDesc()
-    d.q, d.q_row_stride, d.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    d.pages, d.n_pages, d.kv_heads, d.hd = pages.data_ptr(), n_pages, kv_heads, hd
-    d.tables, d.table_stride, d.width, d.lens = tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr()
-    d.rows, d.heads, d.scale, d.alibi_slopes = rows, heads, scale, _p(alibi)
-    d.out, d.o_row_stride, d.o_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-    d.group, d.shared_len = (group, shared_len.data_ptr()) if group > 1 and shared_len is not None else (1, None)
-    L = _lib.lib()
-    n = L.unimp_kv4_attn_workspace(C.byref(d))
-    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None          # of this call: nothing that two streams or graphs could share
-    check(L.unimp_kv4_attn_decode(C.byref(d), _p(ws), _stream()), "kv4_attn_decode")
+        out = torch.empty(q.shape, dtype=bf16, device=q.device)
+    grouped = group > 1 and shared_len is not None
+    if not (q.dim() == 3 and q.dtype is bf16 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous() and pages.shape[2] == _KV4_BYTES.get(q.shape[2])
+            and pages.shape[0] > 0 and pages.shape[1] > 0 and q.shape[1] % pages.shape[1] == 0 and q.shape[1] <= 16 * pages.shape[1]
+            and tables.dim() == 2 and tables.dtype is _i32 and tables.shape[0] == q.shape[0] and tables.stride(1) == 1
+            and lens.dtype is _i32 and lens.shape == (q.shape[0],) and lens.is_contiguous()
+            and (alibi is None or (alibi.dtype is _f32 and alibi.shape == (q.shape[1],) and alibi.is_contiguous()))
+            and (shared_len is None or (group >= 1 and q.shape[0] % group == 0 and shared_len.dtype is _i32 and shared_len.shape == (q.shape[0] // group,) and shared_len.is_contiguous()))
+            and out.dtype is bf16 and out.shape == q.shape and out.stride(2) == 1):
+        _kv4_refuse("kv4_attn_decode", "q and out bf16 [rows, heads, hd]; pages contiguous uint8 [n_pages, kv heads, kv4_page_bytes(hd)], heads a multiple of kv heads, at most 16 to one; "
+                    "tables int32 [rows, width] with unit column stride; lens contiguous int32 [rows]; alibi contiguous fp32 [heads]; shared_len contiguous int32 [rows // group]",
+                    q=q, pages=pages, tables=tables, lens=lens, alibi=alibi, group=group, shared_len=shared_len, out=out)
+    q = _kv4_rows(q)
+    (rows, heads, hd), (qr, qh, _), (o_r, o_h, _) = q.shape, q.stride(), out.stride()
+    n_pages, kv_heads, _ = pages.shape
+    width = tables.shape[1]
+    n = _kv4_workspace(rows, heads, kv_heads, hd, width, group if grouped else 1)
+    ws = torch.empty(n, dtype=_f32, device=q.device) if n else None                   # of this call: nothing that two streams or graphs could share
+    d = _KV4_ATTN.pack(q.data_ptr(), qr, qh, pages.data_ptr(), n_pages, kv_heads, hd, tables.data_ptr(), tables.stride(0), width, lens.data_ptr(), rows, heads, scale,
+                       0 if alibi is None else alibi.data_ptr(), out.data_ptr(), o_r, o_h, group if grouped else 1, shared_len.data_ptr() if grouped else 0)
+    _kv4_launch(_lib.lib().unimp_kv4_attn_decode, "kv4_attn_decode", (q, pages, tables, lens, out, alibi, shared_len), (d, ws.data_ptr() if n else None))
     return out
