@@ -7,6 +7,8 @@ as ONE HIP graph: the position lives on the device (functional.StepState), every
 the beam reorder of the generated K/V tail is part of the graph.  The host only writes the new tokens / source rows and
 reads the logits.
 """
+import weakref
+
 import torch
 
 from . import functional as F_
@@ -14,8 +16,10 @@ from . import ops
 
 
 # step signatures that have run eagerly once in this process: everything lazy behind them (live GEMM tuning, kernel attributes, the decode attention's
-# workspace) exists, so a later session of the same signature captures its FIRST step instead of running it eagerly (8 - 10 ms per generate() call)
-_WARM = set()
+# workspace) exists, so a later session of the same signature captures its FIRST step instead of running it eagerly (8 - 10 ms per generate() call).  Kept per
+# model OBJECT, not per id(): the id of a collected model comes back for the next one, whose first step was then captured cold (a rotary table copied to the device inside
+# the capture: hipErrorStreamCaptureUnsupported)
+_WARM = weakref.WeakKeyDictionary()
 
 
 class DecodeSession:
@@ -66,6 +70,8 @@ class DecodeSession:
         c.len = Lmax                             # capacity bookkeeping on the host; the rows' true lengths live in StepState
         c.row_len = None
         self.cache, self.Lmax = c, Lmax
+        if hasattr(self.lm, "_rope_tables"):     # the rows of every position this session can reach, before any step is captured (a warm signature fixes the capacity
+            self.lm._rope_tables(c.kv.shape[3], dev)      # only up to 128 slots: a longer session of it may need rows that the tower does not have yet)
         c.media_count = ((prompts == m.media_token_id) & (torch.arange(Lmax, device=dev)[None, :] < row_len[::K, None])) \
             .sum(1, keepdim=True).to(torch.int32).repeat_interleave(K, 0)
         c.step = F_.StepState(R, row_len, dev)
@@ -106,13 +112,13 @@ class DecodeSession:
         # what the lazily created state depends on: the model, the rows, the head geometry and the number of 128-key chunks of the cache (the decode
         # attention's workspace) -- not the exact capacity, so prompts of other lengths in the same chunk count are warm as well
         kvs = c.kv.shape
-        sig = (id(self.model), kvs[0], kvs[2], (kvs[3] + 127) // 128, kvs[4], kvs[5], self.beams, bool(self.reorder), F_.DECODE_FUSED, F_.DECODE_STEP_ATTN,
+        sig = (kvs[0], kvs[2], (kvs[3] + 127) // 128, kvs[4], kvs[5], self.beams, bool(self.reorder), F_.DECODE_FUSED, F_.DECODE_STEP_ATTN,
                F_.DECODE_STEP_GROUPED)
         if not self.use_graph:
             logits = self._step_body()
-        elif self.graph is None and sig not in _WARM:
+        elif self.graph is None and sig not in _WARM.get(self.model, ()):
             logits = self._step_body()          # first step of this signature eagerly: warms every lazy initialisation outside the capture
-            _WARM.add(sig)
+            _WARM.setdefault(self.model, set()).add(sig)
         else:
             if self.graph is None:
                 self.graph = torch.cuda.CUDAGraph()

@@ -1165,7 +1165,8 @@ def kv4_read(pages, slots, hd):
         _kv4_refuse("kv4_read", "pages uint8 [(layers,) n_pages, heads, kv4_page_bytes(hd)], every layer contiguous; slots contiguous int64 [tokens]", pages=pages, slots=slots, hd=hd)
     tokens, (n_pages, heads) = slots.shape[0], pages.shape[-3:-1]
     shape = (*pages.shape[:-3], tokens, heads, hd)
-    k, v = torch.empty(shape, dtype=bf16, device=pages.device), torch.empty(shape, dtype=bf16, device=pages.device)
+    k = pages.new_empty(shape, dtype=bf16)
+    v = torch.empty_like(k)
     _kv4_launch(_lib.lib().unimp_kv4_read, "kv4_read", (pages, slots), (pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr()))
     return k, v
 
@@ -1187,8 +1188,7 @@ def page_tables_extend(tables, mapped, cached, new, free_pages, cursor, max_toke
         _kv4_refuse("page_tables_extend", "contiguous int32: tables [rows, width], mapped, cached, new, cover [rows], free_pages [n], cursor [1], shared_len [rows // group]; rows a multiple "
                     "of group", tables=tables, mapped=mapped, cached=cached, new=new, cover=cover, free_pages=free_pages, cursor=cursor, group=group, shared_len=shared_len,
                     max_tokens=max_tokens)
-    dev = tables.device
-    ints, slots = torch.empty(2 * rows + 2, dtype=_i32, device=dev), torch.empty(max_tokens, dtype=_i64, device=dev)
+    ints, slots = tables.new_empty(2 * rows + 2), tables.new_empty(max_tokens, dtype=_i64)
     p = ints.data_ptr()                                       # mapped [rows], cursor [1], cu [rows + 1]
     _kv4_launch(_lib.lib().unimp_page_tables_extend, "page_tables_extend", (tables, mapped, cached, new, free_pages, cursor, cover, shared_len),
                 (tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), None if cover is None else cover.data_ptr(), free_pages.data_ptr(),
@@ -1232,7 +1232,7 @@ def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_l
     row of length 0 gives zeros; a page id outside the pool hides its tokens.  group > 1 with shared_len (int32 [rows // group]): the rows of a group (the beams of a
     prompt) name the same pages below shared_len // 32 columns; those are read once per group.  Returns o [rows, heads, hd]."""
     if out is None:
-        out = torch.empty(q.shape, dtype=bf16, device=q.device)
+        out = q.new_empty(q.shape)
     grouped = group > 1 and shared_len is not None
     if not (q.dim() == 3 and q.dtype is bf16 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous() and pages.shape[2] == _KV4_BYTES.get(q.shape[2])
             and pages.shape[0] > 0 and pages.shape[1] > 0 and q.shape[1] % pages.shape[1] == 0 and q.shape[1] <= 16 * pages.shape[1]
@@ -1249,7 +1249,7 @@ def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_l
     n_pages, kv_heads, _ = pages.shape
     width = tables.shape[1]
     n = _kv4_workspace(rows, heads, kv_heads, hd, width, group if grouped else 1)
-    ws = torch.empty(n, dtype=_f32, device=q.device) if n else None                   # of this call: nothing that two streams or graphs could share
+    ws = q.new_empty(n, dtype=_f32) if n else None                   # of this call: nothing that two streams or graphs could share
     d = _KV4_ATTN.pack(q.data_ptr(), qr, qh, pages.data_ptr(), n_pages, kv_heads, hd, tables.data_ptr(), tables.stride(0), width, lens.data_ptr(), rows, heads, scale,
                        0 if alibi is None else alibi.data_ptr(), out.data_ptr(), o_r, o_h, group if grouped else 1, shared_len.data_ptr() if grouped else 0)
     _kv4_launch(_lib.lib().unimp_kv4_attn_decode, "kv4_attn_decode", (q, pages, tables, lens, out, alibi, shared_len), (d, ws.data_ptr() if n else None))
