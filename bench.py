@@ -721,7 +721,7 @@ def main():
     if prof is None:
         prof, ops.GEMM_PROFILE = ops.GEMM_PROFILE, None
     if world > 1:
-        t = torch.tensor([dt], device=dev, dtype=torch.float64)
+        t = torch.tensor([dt], device=dev if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         dt = t.item()
     ms = dt / args.steps * 1e3
@@ -749,7 +749,7 @@ def main():
             torch.cuda.synchronize()
             dtp = time.perf_counter() - tp0
             if world > 1:
-                t = torch.tensor([dtp], device=dev, dtype=torch.float64)
+                t = torch.tensor([dtp], device=dev if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
                 dist.all_reduce(t, op=dist.ReduceOp.MAX)
                 dtp = t.item()
             packed_leg = {"value": round(B * world * kp / dtp, 3), "unit": "samples/s", "ms_per_step": round(dtp / kp * 1e3, 2), "steps": kp, "warmup": 4,

@@ -22,6 +22,8 @@ enough to be link-bandwidth- rather than latency-bound.
 import torch
 import torch.distributed as dist
 
+from . import hostcomm
+
 
 class GradBucketer:
     def __init__(self, optimizer, bucket_bytes=256 << 20, process_group=None, late_params=(), force_hooks=False):
@@ -136,7 +138,7 @@ class GradBucketer:
             lo, hi, _ = self.opt.owned[bi]
             self._handles.append(dist.reduce_scatter_tensor(g[lo:hi], g[s:e], op=dist.ReduceOp.SUM, group=self.pg, async_op=True))
         else:       # replicated state, or a backend without reduce-scatter (gloo in the tests): the owned slice of the sum is what is used
-            self._handles.append(dist.all_reduce(g[s:e], op=dist.ReduceOp.SUM, group=self.pg, async_op=True))
+            self._handles.append(hostcomm.all_reduce(g[s:e], dist.ReduceOp.SUM, self.pg, async_op=True))
 
     def finish(self):
         """call after backward: issue, in index order, the buckets that did not go out during backward (parameters

@@ -1,0 +1,39 @@
+"""Collectives for a backend that moves host memory (gloo: CPU runs, and several ranks that share one GPU).  A device tensor is staged through host memory with synchronous
+copies: gloo's own device path works on streams of another priority and has hung where several ranks shared a card.  RCCL never comes here."""
+import torch
+import torch.distributed as dist
+
+
+def staged(t, group):
+    """does a collective of ``group`` on ``t`` go through host memory?"""
+    return t.is_cuda and dist.get_backend(group) != "nccl"
+
+
+class _Staged:
+    """handle of an asynchronous all-reduce of a host copy; the sum reaches the device tensor in wait()"""
+
+    def __init__(self, t, op, group):
+        self.t, self.host = t, t.to("cpu")                    # synchronous: every kernel that writes t has finished
+        self.work = dist.all_reduce(self.host, op=op, group=group, async_op=True)
+
+    def wait(self):
+        self.work.wait()
+        self.t.copy_(self.host)
+
+
+def all_reduce(t, op, group, async_op=False):
+    """in place; returns a handle if async_op"""
+    if not staged(t, group):
+        return dist.all_reduce(t, op=op, group=group, async_op=async_op)
+    h = _Staged(t, op, group)
+    if async_op:
+        return h
+    h.wait()
+
+
+def all_gather_cat(out, mine, world, group):
+    """out [world * n] = the ranks' ``mine`` [n] in rank order"""
+    src = mine.to("cpu") if staged(mine, group) else mine.contiguous()
+    parts = [torch.empty_like(src) for _ in range(world)]
+    dist.all_gather(parts, src, group=group)
+    out.copy_(torch.cat(parts))

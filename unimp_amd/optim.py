@@ -10,7 +10,7 @@ Decay grouping reproduces the reference filter, including its ``ff.0.weight`` qu
 import math
 import torch
 
-from . import ops
+from . import hostcomm, ops
 
 
 def apply_decay(name):
@@ -153,7 +153,7 @@ class FlatAdamW:
         # the owned slices hold the reduce-scattered (summed) gradient: their squares add up, over the ranks, to the global norm
         for lo, hi, so in self.owned:
             ops.sumsq(self.flat_g[lo:hi], self.norm_buf)
-        dist.all_reduce(self.norm_buf[0:1], op=dist.ReduceOp.SUM, group=pg)
+        hostcomm.all_reduce(self.norm_buf[0:1], dist.ReduceOp.SUM, pg)
         for lo, hi, so in self.owned:
             k = hi - lo
             ops.adamw_flat(self.master[so:so + k], self.m[so:so + k], self.v[so:so + k], self.flat_p[lo:hi], self.flat_g[lo:hi],
@@ -165,10 +165,8 @@ class FlatAdamW:
         for (s_, e_), (lo, hi, so) in zip(self.buckets, self.owned):
             if nccl:
                 dist.all_gather_into_tensor(self.flat_p[s_:e_], self.flat_p[lo:hi], group=pg)
-            else:       # gloo (tests): list form through a temporary
-                parts = [torch.empty_like(self.flat_p[lo:hi]) for _ in range(self.shard[1])]
-                dist.all_gather(parts, self.flat_p[lo:hi].contiguous(), group=pg)
-                self.flat_p[s_:e_].copy_(torch.cat(parts))
+            else:
+                hostcomm.all_gather_cat(self.flat_p[s_:e_], self.flat_p[lo:hi], self.shard[1], pg)
 
     def grad_norm(self):
         """device scalar: global L2 norm of the gradient the last step() clipped -- the averaged one, i.e. the summed
@@ -198,9 +196,7 @@ class FlatAdamW:
             if nccl:
                 dist.all_gather_into_tensor(full[s_:e_], mine, group=pg)
             else:
-                parts = [torch.empty_like(mine) for _ in range(w)]
-                dist.all_gather(parts, mine, group=pg)
-                full[s_:e_].copy_(torch.cat(parts))
+                hostcomm.all_gather_cat(full[s_:e_], mine, w, pg)
         return full
 
     def state_dict(self, to_host=True):
