@@ -131,3 +131,13 @@ def test_packed_descriptor_is_the_struct():
     assert len(packed) == C.sizeof(d) or len(packed) == C.sizeof(d) - C.sizeof(d) % 8
     again = _lib.Kv4AttnDesc.from_buffer_copy(packed.ljust(C.sizeof(d), b"\0"))
     assert [getattr(again, n) for n, _ in d._fields_] == vals
+
+
+def test_decode_session_refuses_other_caches():
+    from types import SimpleNamespace
+    from unimp_amd.decode import DecodeSession
+    from unimp_amd.functional import Kv4Cache
+    with pytest.raises(ValueError):
+        DecodeSession(SimpleNamespace(lang_encoder=None), 4, False, kv_cache="int8")
+    with pytest.raises(ValueError):
+        Kv4Cache(SimpleNamespace(layers=[], kv=torch.zeros(1, 2, 1, 8, 2, 64, dtype=bf16)), [8], beams=17, max_new=4)

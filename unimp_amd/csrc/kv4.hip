@@ -188,57 +188,71 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
 }
 
 // ------------------------------------------------------------------------------------------- decode step: rotary embedding + append
-// Block (row, head): thread d holds dim d of q, k and v.  The rotation runs in 64 bits (two products of a bf16 and an fp32, exact there): a code is decided
-// next to a border, and k's codes are those of the exact rotation of the given tables.  The nibbles of V go in by atomics: two rows of a launch may write
-// different tokens of one page.
+// A wave per (row, head), two dims to a lane.  The rotation runs in 64 bits (two products of a bf16 and an fp32, exact there): a code is decided next to a border, and
+// k's codes are those of the exact rotation of the given tables.  V's nibbles go in by atomics: two rows of a launch may write different tokens of one page.  Bound by its
+// three dependent steps (load, block maximum, write), not by bytes.
 __device__ __forceinline__ uint32_t kv4_code_f64(double x, double inv) {
   const double a = fabs(x) * inv;
   const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
   return c | (x < 0.0 ? 8u : 0u);
 }
+template <int CTRL> __device__ __forceinline__ int kv4_dpp(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true); }
 template <int D>
-__global__ __launch_bounds__(128) void kv4_rope_append_kernel(const bf16* __restrict__ qkv, long row_stride, long head_stride, int q_off, int k_off, int v_off,
+__global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __restrict__ qkv, long row_stride, long head_stride, int q_off, int k_off, int v_off,
                                                               int rot, const float* __restrict__ cos_rows, const float* __restrict__ sin_rows,
                                                               bf16* __restrict__ q_out, uint8_t* __restrict__ pages, long n_pages, int heads,
                                                               const int64_t* __restrict__ slots) {
   using P = Kv4<D>;
-  const int row = blockIdx.y, head = blockIdx.x, d = threadIdx.x;
-  const bf16* base = qkv + (long)row * row_stride + (long)head * head_stride;
-  double q = 0, k = 0, v = 0;
-  if (d < D) {
-    q = (double)bf2f(base[q_off + d]); k = (double)bf2f(base[k_off + d]); v = (double)bf2f(base[v_off + d]);
-    if (d < rot) {
-      const int h = rot >> 1, i = d < h ? d : d - h, p = d < h ? d + h : d - h;
-      const double c = cos_rows[(long)row * h + i], s = sin_rows[(long)row * h + i];
-      const double q2 = (double)bf2f(base[q_off + p]), k2 = (double)bf2f(base[k_off + p]);
-      q = d < h ? q * c - q2 * s : q * c + q2 * s;
-      k = d < h ? k * c - k2 * s : k * c + k2 * s;
-    }
-    q_out[((long)row * heads + head) * D + d] = f2bf((float)q);
-  }
+  const int row = blockIdx.y, lane = lane_id(), head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = 2 * lane;
+  if (head >= heads) return;                                        // uniform over the wave
   const int64_t slot = slots[row];
-  if (slot < 0 || slot >= n_pages * KV4_PAGE) return;               // uniform over the block
+  const bf16* base = qkv + (long)row * row_stride + (long)head * head_stride;
+  double q[2] = {0, 0}, k[2] = {0, 0}, v[2] = {0, 0};
+  if (d < D) {
+    const int h = rot >> 1;
+    const float* c = cos_rows + (long)row * h;
+    const float* s = sin_rows + (long)row * h;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = d + j;
+      q[j] = (double)bf2f(base[q_off + e]); k[j] = (double)bf2f(base[k_off + e]); v[j] = (double)bf2f(base[v_off + e]);
+      if (e < rot) {
+        const int i = e < h ? e : e - h, p = e < h ? e + h : e - h;
+        const double cc = c[i], ss = s[i], q2 = (double)bf2f(base[q_off + p]), k2 = (double)bf2f(base[k_off + p]);
+        q[j] = e < h ? q[j] * cc - q2 * ss : q[j] * cc + q2 * ss;
+        k[j] = e < h ? k[j] * cc - k2 * ss : k[j] * cc + k2 * ss;
+      }
+    }
+    bf16x2 o = {f2bf((float)q[0]), f2bf((float)q[1])};
+    *(bf16x2*)(q_out + ((long)row * heads + head) * D + d) = o;
+  }
+  if (slot < 0 || slot >= n_pages * KV4_PAGE) return;               // uniform
   const int t = (int)(slot & 31);
   uint8_t* page = pages + ((slot >> 5) * heads + head) * (long)P::BYTES;
-  uint32_t code[2]; int sb[2];
+  uint32_t code[2][2]; int sb[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const double x = w ? v : k;
-    int e = (int)((__double2hiint(x) >> 20) & 0x7ff);               // exponent field: floor(log2 |x|) + 1023, 2047 for infinity and NaN
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) e = max(e, __shfl_xor(e, o, 32));
+    const double (&x)[2] = w ? v : k;
+    // exponent field: floor(log2 |x|) + 1023, 2047 for infinity and NaN; its maximum over the 16 lanes of a block
+    int e = max((int)((__double2hiint(x[0]) >> 20) & 0x7ff), (int)((__double2hiint(x[1]) >> 20) & 0x7ff));
+    e = max(e, kv4_dpp<0xB1>(e)); e = max(e, kv4_dpp<0x4E>(e));     // lane ^ 1, ^ 2: quads agree
+    e = max(e, kv4_dpp<0x141>(e)); e = max(e, kv4_dpp<0x140>(e));   // mirrored inside 8 and inside 16 lanes
     sb[w] = e == 2047 ? 255 : max(e - 1023 - 2, -125) + 127;
-    code[w] = sb[w] == 255 ? 0u : kv4_code_f64(x, __hiloint2double((1023 + 127 - sb[w]) << 20, 0));
-  }
-  uint32_t kk = code[0] << (4 * (d & 7));                           // eight lanes' K codes into one dword
+    const double inv = __hiloint2double((1023 + 127 - sb[w]) << 20, 0);
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) kk |= __shfl_xor(kk, o, 8);
+    for (int j = 0; j < 2; ++j) code[w][j] = sb[w] == 255 ? 0u : kv4_code_f64(x[j], inv);
+  }
+  int kk = (int)((code[0][0] | (code[0][1] << 4)) << (8 * (lane & 3)));      // four lanes' K codes into one dword
+  kk |= kv4_dpp<0xB1>(kk); kk |= kv4_dpp<0x4E>(kk);
   if (d < D) {
-    if (!(d & 7)) *(uint32_t*)(page + P::k_byte(t, d >> 5) + ((d & 31) >> 1)) = kk;
-    if (!(d & 31)) { page[P::ks_byte(t, d >> 5)] = (uint8_t)sb[0]; page[P::vs_byte(t, d >> 5)] = (uint8_t)sb[1]; }
-    uint32_t* o = (uint32_t*)(page + P::v_dword(t, d));
+    if (!(lane & 3)) *(uint32_t*)(page + P::k_byte(t, d >> 5) + ((d & 31) >> 1)) = (uint32_t)kk;
+    if (!(lane & 15)) { page[P::ks_byte(t, d >> 5)] = (uint8_t)sb[0]; page[P::vs_byte(t, d >> 5)] = (uint8_t)sb[1]; }
     const int sh = 4 * kv4_nibble(t);
-    atomicAnd(o, ~(15u << sh)); atomicOr(o, code[1] << sh);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t* o = (uint32_t*)(page + P::v_dword(t, d + j));
+      atomicAnd(o, ~(15u << sh)); atomicOr(o, code[1][j] << sh);
+    }
   }
 }
 
@@ -247,9 +261,9 @@ extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_
   if (!qkv || !q_out || !pages || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
   if (rows <= 0 || heads <= 0) return UNIMP_OK;
   if (rot < 0 || (rot & 1) || rot > hd || rows > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_rope_append: rot even and at most the head dim, at most 65535 rows");
-  if ((uintptr_t)pages & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_rope_append: 16-byte aligned pages");
+  if (((uintptr_t)pages & 15) || ((uintptr_t)q_out & 3)) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_rope_append: 16-byte aligned pages, 4-byte aligned q_out");
   return kv4_for_hd(hd, [&](auto d) {
-    hipLaunchKernelGGL((kv4_rope_append_kernel<decltype(d)::value>), dim3(heads, rows), dim3(128), 0, (hipStream_t)stream, (const bf16*)qkv, (long)row_stride,
+    hipLaunchKernelGGL((kv4_rope_append_kernel<decltype(d)::value>), dim3((heads + 3) / 4, rows), dim3(256), 0, (hipStream_t)stream, (const bf16*)qkv, (long)row_stride,
                        (long)head_stride, q_off, k_off, v_off, rot, cos_rows, sin_rows, (bf16*)q_out, (uint8_t*)pages, (long)n_pages, heads, slots);
     return unimp_check_launch("kv4_rope_append");
   });
@@ -368,16 +382,23 @@ __device__ __forceinline__ PageRow page_row(const PageArgs& a, int r, int& alias
   }
   return PageRow{need, max(map, alias)};
 }
-__global__ __launch_bounds__(256) void page_tables_extend_kernel(PageArgs a) {
+#define PAGE_T 256
+__global__ __launch_bounds__(PAGE_T) void page_tables_extend_kernel(PageArgs a) {
   __shared__ long red[3][4];
   const int r = blockIdx.x, tid = threadIdx.x, first = a.group > 1 ? r / a.group * a.group : r;
   const bool last = r == a.rows - 1;
   long before = 0, before_first = 0, tok = 0;
-  for (int i = tid; i < r; i += 256) {
-    int al, m; const PageRow p = page_row(a, i, al, m);
-    const int own = max(p.need - p.begin, 0);
-    before += own; tok += max(a.fresh[i], 0);
-    if (i < first) before_first += own;
+  if (!a.shared) {                                                   // no groups: the loads of eight rows at once
+#pragma unroll 8
+    for (int i = tid; i < r; i += PAGE_T) { int m; const int need = page_need(a, i, m); before += max(need - m, 0); tok += max(a.fresh[i], 0); }
+    before_first = before;
+  } else {
+    for (int i = tid; i < r; i += PAGE_T) {
+      int al, m; const PageRow p = page_row(a, i, al, m);
+      const int own = max(p.need - p.begin, 0);
+      before += own; tok += max(a.fresh[i], 0);
+      if (i < first) before_first += own;
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) { before += __shfl_xor(before, o, 64); before_first += __shfl_xor(before_first, o, 64); tok += __shfl_xor(tok, o, 64); }
@@ -399,16 +420,16 @@ __global__ __launch_bounds__(256) void page_tables_extend_kernel(PageArgs a) {
     return c < p.need ? from_free(before + c - p.begin) : -1;
   };
   const int n = max(a.fresh[r], 0), have = max(a.cached[r], 0);
-  for (long t = tid; t < n && tok + t < a.max_tokens; t += 256) {
+  for (long t = tid; t < n && tok + t < a.max_tokens; t += PAGE_T) {
     const long pos = (long)have + t, c = pos / KV4_PAGE;
     const long page = c < a.width ? (long)lookup((int)c) : -1;
     a.slots[tok + t] = page >= 0 ? page * KV4_PAGE + (pos & 31) : -1;
   }
-  for (int c = map + tid; c < p.need; c += 256) row[c] = lookup(c);
+  for (int c = map + tid; c < p.need; c += PAGE_T) row[c] = lookup(c);
   if (tid == 0) { a.mapped_out[r] = max(map, p.need); a.cu[r] = (int)tok; }
   if (last) {
     if (tid == 0) { a.cu[a.rows] = (int)(tok + n); a.cursor_out[0] = (int)(before + max(p.need - p.begin, 0)); }
-    for (long i = tok + n + tid; i < a.max_tokens; i += 256) a.slots[i] = -1;
+    for (long i = tok + n + tid; i < a.max_tokens; i += PAGE_T) a.slots[i] = -1;
   }
 }
 
@@ -421,7 +442,7 @@ extern "C" int unimp_page_tables_extend(int32_t* tables, int rows, int width, co
     return unimp_set_error(UNIMP_ERR_SHAPE, "page_tables_extend: rows a positive multiple of group, width positive");
   if (mapped == mapped_out || cursor == cursor_out) return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: the blocks read mapped and cursor throughout; outputs of their own");
   PageArgs a{tables, mapped, cached, fresh, cover, free_pages, cursor, shared_len, mapped_out, cursor_out, cu, slots, (long)max_tokens, rows, width, n_free, group};
-  hipLaunchKernelGGL(page_tables_extend_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(page_tables_extend_kernel, dim3(rows), dim3(PAGE_T), 0, (hipStream_t)stream, a);
   return unimp_check_launch("page_tables_extend");
 }
 

@@ -262,7 +262,9 @@ class Flamingo(nn.Module):
         then greedy / beam search over the LM (generate.py: transformers' BeamSearchScorer semantics).  ``use_cache=True``
         (transformers' default) decodes with the KV cache: one prefill over the prompt, then one token per row and step,
         the cache rows following their beams, the step replayed as a HIP graph (decode.py; ``use_graph=False`` launches it
-        kernel by kernel); ``use_cache=False`` re-scores the full sequences every step."""
+        kernel by kernel); ``use_cache=False`` re-scores the full sequences every step.  ``kv_cache="mx4"`` keeps the cached K / V on 4-bit
+        pages (about a quarter of the bytes; the beams of a prompt share its pages): for long prompts, many beams or many users per call.  The
+        generated tokens are those of keys and values rounded to 4 bits, not the bf16 cache's."""
         from .generate import beam_search, greedy_search
         from .decode import DecodeSession
         num_beams = kwargs.pop("num_beams", 1)
@@ -277,9 +279,12 @@ class Flamingo(nn.Module):
         lp = kwargs.pop("length_penalty", 1.0)
         use_cache = kwargs.pop("use_cache", True)
         use_graph = kwargs.pop("use_graph", True)      # replay the decode step as one HIP graph (decode.py)
+        kv_cache = kwargs.pop("kv_cache", "bf16")      # "mx4": K / V of the decode on 4-bit pages (functional.Kv4Cache)
         trace = kwargs.pop("trace", None)              # tests: per-step candidate scores of the beam search
         if kwargs.pop("do_sample", False) or kwargs:
             raise NotImplementedError(f"unsupported generate() arguments: do_sample / {sorted(kwargs)}")
+        if kv_cache not in ("bf16", "mx4") or (kv_cache != "bf16" and not use_cache):
+            raise ValueError(f"generate(): kv_cache {kv_cache!r}: 'bf16', or 'mx4' with use_cache=True")
         was_training = self.training
         self.eval()
         lengths, seqs0 = None, lang_x
@@ -307,7 +312,7 @@ class Flamingo(nn.Module):
                     self._condition_media_locations(input_ids=seqs)
                     return self.lang_encoder(input_ids=seqs, attention_mask=None, logits_last_only=True)["logits"][:, -1]
                 if session[0] is None:
-                    session[0] = DecodeSession(self, max_new_tokens, reorder=num_beams > 1, graph=use_graph, beams=num_beams)
+                    session[0] = DecodeSession(self, max_new_tokens, reorder=num_beams > 1, graph=use_graph, beams=num_beams, kv_cache=kv_cache)
                     return session[0].prefill(lang_x, lengths)
                 return session[0].step(seqs[:, -1], src)
             if num_beams > 1:

@@ -710,11 +710,12 @@ def linear_ln(x, ln_w, ln_b, eps, w, ldc=None):
 class LayerKV:
     """decode state of one decoder layer: views ``k``, ``v`` [rows, capacity, nh, hd] into the cache's single K/V tensor
     (keys after RoPE) and the gated cross-attention's projected media ``xkv`` [rows, T*n, 2*inner] (constant over a decode)."""
-    __slots__ = ("owner", "k", "v", "xkv")
+    __slots__ = ("owner", "k", "v", "xkv", "pages")
 
     def __init__(self, owner):
         self.owner = weakref.proxy(owner)      # no DecodeCache <-> LayerKV cycle: the K/V tensor must die with its last user, not at the next gc pass
         self.k = self.v = self.xkv = None
+        self.pages = None                      # Kv4Cache: this layer's pool [n_pages, heads, page bytes] instead of k / v
 
 
 class StepState:
@@ -779,6 +780,56 @@ class DecodeCache:
             self.media_count = self.media_count.index_select(0, idx)
 
 
+class Kv4Cache(DecodeCache):
+    """the decode state with K / V on 4-bit pages (ops.kv4_*): ``pages`` uint8 [layers, n_pages, heads, page bytes], ``tables`` int32 [rows, columns] naming each row's
+    pages (32 tokens each, the same for all layers).  The rows of a beam group share the pages of their prompt; every row has pages of its own from the one that its first
+    generated token goes to.  Made of a finished prefill's bf16 cache: 17 / 64 of its bytes per token, the prompt once instead of once per beam."""
+
+    def __init__(self, prompts, host_len, beams, max_new):
+        """prompts: the prefill's DecodeCache (one row per prompt); host_len: the prompts' lengths; max_new: tokens that every row may still take"""
+        super().__init__(len(prompts.layers))
+        _, _, B, cap, nh, hd = prompts.kv.shape
+        if beams > 16:
+            raise ValueError(f"the 4-bit cache holds at most 16 beams of a prompt, not {beams}")
+        dev, K, P = prompts.kv.device, beams, ops.KV4_PAGE
+        cols = [-(-(n + max_new) // P) for n in host_len]
+        n_pages = sum(c + (K - 1) * (c - n // P) for c, n in zip(cols, host_len))
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+        self.pages = torch.empty((len(prompts.layers), n_pages, nh, ops.kv4_page_bytes(hd)), dtype=torch.uint8, device=dev)
+        self.tables = torch.full((B * K, max(cols)), -1, dtype=torch.int32, device=dev)
+        self.group, self.shared_len = K, i32(host_len) if K > 1 else None
+        self.free, self.ones = torch.arange(n_pages, dtype=torch.int32, device=dev), torch.ones(B * K, dtype=torch.int32, device=dev)
+        length = i32(host_len).repeat_interleave(K)
+        first = (torch.arange(B * K, device=dev) % K == 0).to(torch.int32)
+        zero = torch.zeros(B * K, dtype=torch.int32, device=dev)
+        self.mapped, self.cursor, slots, cu = ops.page_tables_extend(self.tables, zero, zero, length * first, self.free, zero[:1], sum(host_len), cover=length + max_new,
+                                                                     group=K, shared_len=self.shared_len)
+        t = torch.arange(cap, device=dev)                      # the packed tokens' slots, spread to the padded rows of the prefill's cache
+        at = (cu[:-1:K].long()[:, None] + t).clamp_(max=sum(host_len) - 1)
+        slots = torch.where(t < length[::K, None], slots[at], torch.full((), -1, dtype=torch.long, device=dev)).reshape(-1)
+        for lk, lp, pages in zip(self.layers, prompts.layers, self.pages):
+            lk.pages = pages
+            ops.kv4_write(lp.k.view(B * cap, nh, hd), lp.v.view(B * cap, nh, hd), pages, slots)
+        self.cached = length                                    # tokens in the cache, per row
+        self.slots = None                                       # of the step's new tokens
+        if K > 1:                                               # the page in which a prompt ends: every beam goes on in its own copy
+            self.reorder_beams(torch.zeros(B * K, dtype=torch.long, device=dev), length.long())
+
+    def reorder(self, idx):
+        raise NotImplementedError("Kv4Cache: beams are reordered inside their groups (reorder_beams)")
+
+    def reorder_beams(self, src_local, pos):
+        """row j of every group goes on with the hypothesis of row src_local of its group (index inside the group); pos int64 [rows] = tokens cached"""
+        ops.kv4_reorder_beams(self.pages, self.tables, self.group, src_local, pos)
+
+    def begin_step(self):
+        """the slots of the step's new tokens, one per row, from the rows' lengths (every column is mapped from the start: nothing is taken from the free list)"""
+        self.slots = ops.page_tables_extend(self.tables, self.mapped, self.cached, self.ones, self.free, self.cursor, self.tables.shape[0])[2]
+
+    def end_step(self):
+        self.cached.add_(1)
+
+
 def _kv_append(lc, k, v, pos0):
     need = pos0 + k.shape[1]
     lc.owner._reserve(k, need)
@@ -826,6 +877,11 @@ def self_attn_block_cached(x, ln_w, ln_b, wqkv, bqkv, wd, bd, nh, lc, pos0, *, r
             raise NotImplementedError("a static decode step feeds one new token per row")
         rot = rope[2] if rope is not None else 0
         o3 = (offs[0], offs[1], (2 * hd) if interleaved else 2 * H)       # q, k, v element offsets inside a head slot (_split_qkv)
+        if lc.pages is not None:               # 4-bit pages: rotate + quantise + append, then the attention over the pages
+            own = lc.owner
+            q = ops.kv4_rope_append(qkv, nh, hs, hd, o3, rot, rope[0] if rot else None, rope[1] if rot else None, lc.pages, own.slots)
+            o = ops.kv4_attn_decode(q, lc.pages, own.tables, step.kv_len, scale, alibi, own.group, own.shared_len)
+            return ops.gemm(o.view(R, H), wd, bias=bd, res=r2).view(R, 1, H)
         fused = DECODE_FUSED and qk_ln is None and ops.decode_rope_append_ok(hd, rot, hs, o3, qkv, lc.k)
         if fused and DECODE_STEP_ATTN and ops.DECODE_ATTN and hd <= 128:
             # the whole attention in ONE launch: rope of the new q / k, the append, every cached key (csrc/decode_attn.hip attn_decode_step_kernel);
