@@ -204,6 +204,9 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
                                                               const int64_t* __restrict__ slots) {
   using P = Kv4<D>;
   const int row = blockIdx.y, lane = lane_id(), head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = 2 * lane;
+  // V: dims 32 b + c and 32 b + 16 + c of lane (b, c) are neighbouring dwords: one 64-bit atomic for both (head dim 80: odd rows of dwords, two of 32 bits)
+  constexpr bool PAIR = P::NI % 2 == 0;
+  const int v_dim = PAIR ? 32 * (lane >> 4) + (lane & 15) : d;
   if (head >= heads) return;                                        // uniform over the wave
   const int64_t slot = slots[row];
   const bf16* base = qkv + (long)row * row_stride + (long)head * head_stride;
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int e = d + j;
-      q[j] = (double)bf2f(base[q_off + e]); k[j] = (double)bf2f(base[k_off + e]); v[j] = (double)bf2f(base[v_off + e]);
+      q[j] = (double)bf2f(base[q_off + e]); k[j] = (double)bf2f(base[k_off + e]); v[j] = (double)bf2f(base[v_off + v_dim + 16 * j * PAIR + j * !PAIR]);
       if (e < rot) {
         const int i = e < h ? e : e - h, p = e < h ? e + h : e - h;
         const double cc = c[i], ss = s[i], q2 = (double)bf2f(base[q_off + p]), k2 = (double)bf2f(base[k_off + p]);
@@ -248,10 +251,16 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
     if (!(lane & 3)) *(uint32_t*)(page + P::k_byte(t, d >> 5) + ((d & 31) >> 1)) = (uint32_t)kk;
     if (!(lane & 15)) { page[P::ks_byte(t, d >> 5)] = (uint8_t)sb[0]; page[P::vs_byte(t, d >> 5)] = (uint8_t)sb[1]; }
     const int sh = 4 * kv4_nibble(t);
+    if constexpr (PAIR) {
+      unsigned long long* o = (unsigned long long*)(page + P::v_dword(t, v_dim));
+      const unsigned long long both = 0x100000001ull;
+      atomicAnd(o, ~((15u << sh) * both)); atomicOr(o, (unsigned long long)(code[1][0] << sh) | (unsigned long long)(code[1][1] << sh) << 32);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t* o = (uint32_t*)(page + P::v_dword(t, d + j));
-      atomicAnd(o, ~(15u << sh)); atomicOr(o, code[1][j] << sh);
+      for (int j = 0; j < 2; ++j) {
+        uint32_t* o = (uint32_t*)(page + P::v_dword(t, d + j));
+        atomicAnd(o, ~(15u << sh)); atomicOr(o, code[1][j] << sh);
+      }
     }
   }
 }
