@@ -167,13 +167,13 @@ def tables_ref(tables, mapped, cached, new, cover, free, cursor, group, shared, 
     return tables, out, cur, slots, cu
 
 
-@pytest.mark.parametrize("case", range(12))
+@pytest.mark.parametrize("case", range(15))
 def test_page_tables_extend(ops, case):
     import random
     rng = random.Random(case)
-    group = [1, 1, 1, 5, 10, 2, 1, 3, 1, 1, 4, 1][case]
-    rows = group * [1, 7, 300, 4, 8, 3, 1, 5, 700, 2, 1, 65][case]
-    W = [1, 9, 40, 20, 20, 6, 3, 8, 5, 4, 6, 33][case]
+    group = [1, 1, 1, 5, 10, 2, 1, 3, 1, 1, 4, 1, 1, 7, 1][case]
+    rows = group * [1, 7, 300, 4, 8, 3, 1, 5, 700, 2, 1, 65, 1501, 200, 2][case]
+    W = [1, 9, 40, 20, 20, 6, 3, 8, 5, 4, 6, 33, 7, 5, 900][case]
     cached = [rng.choice([0, 1, 31, 32, 33, rng.randint(0, W * 20)]) if group == 1 else 0 for _ in range(rows)]
     new = [rng.choice([0, 1, 31, 32, rng.randint(0, W * 12)]) for _ in range(rows)]
     if group > 1:
@@ -191,7 +191,7 @@ def test_page_tables_extend(ops, case):
         order = order[:4]                                           # too few pages
     used = sum(mapped)
     tables = [[order[(sum(mapped[:r]) + c) % len(order)] if c < mapped[r] else -1 for c in range(W)] for r in range(rows)]
-    max_tokens = [0, 3, 0, 5, 1, 0, 4, 2, 9, 1, 3, 0][case] + (sum(max(n, 0) for n in new) if case != 11 else 17)
+    max_tokens = [0, 3, 0, 5, 1, 0, 4, 2, 9, 1, 3, 0, 11, 6, 2][case] + (sum(max(n, 0) for n in new) if case != 11 else 17)
     want = tables_ref(tables, mapped, cached, new, cover, order, used, group, shared, max_tokens)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda() if x is not None else None
     tab = i32(tables)
