@@ -398,7 +398,9 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
   p.nw = p.mode == 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
-  p.chunk = clamp((long)d->width * units / 1024, units < 512 ? 4 * p.nw : 64, 64);
+  // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 66.7 us, 48 61.6, 64 67.4, 96 61.8)
+  const int most = d->width <= 64 ? 64 : 48;
+  p.chunk = clamp((long)d->width * units / 1024, units < 512 ? 4 * p.nw : most, most);
   p.chunk_p = p.slots_p = 0;
   if (p.group > 1) {
     p.chunk = 16;
@@ -431,7 +433,8 @@ extern "C" int64_t unimp_kv4_attn_workspace(const unimp_kv4_attn_desc* d) { retu
 template <int D>
 static void kv4_merge_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
   const dim3 grid(a.heads, a.rows);
-  if (p.slots + p.slots_p <= 8) hipLaunchKernelGGL((kv4_attn_merge_kernel<D, 1>), grid, dim3(D / 2), 0, s, a);
+  const int n = p.slots + p.slots_p;                                              // few slots, or enough (row, head) pairs to fill the chip with one wave each
+  if (n <= 8 || (n <= 16 && (long)a.rows * a.heads >= 1024)) hipLaunchKernelGGL((kv4_attn_merge_kernel<D, 1>), grid, dim3(D / 2), 0, s, a);
   else hipLaunchKernelGGL((kv4_attn_merge_kernel<D, 8>), grid, dim3(4 * D), 0, s, a);
 }
 template <int D>
