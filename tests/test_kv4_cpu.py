@@ -108,7 +108,7 @@ def test_c_refusals():
     assert r(k=None) == ARG and r(layers=1 << 17) == r(hd=1) == r(n=1 << 40) == SHAPE and r(k=odd) == ALIGN and r(n=0) == 0
     t = lambda rows=4, width=3, group=1, out=C.c_void_p(1 << 21), cur=C.c_void_p(1 << 22), slots=p, n=5: L.unimp_page_tables_extend(
         p, rows, width, p, p, p, None, p, 9, p, group, None, out, cur, slots, n, p, None)
-    assert t(out=p) == t(cur=p) == t(slots=None) == ARG and t(rows=0) == t(width=0) == t(group=3) == t(group=0) == t(n=-1) == SHAPE
+    assert t(out=p) == t(cur=p) == t(slots=None) == ARG and t(rows=0) == t(rows=65537) == t(width=0) == t(group=3) == t(group=0) == t(n=-1) == SHAPE
     b = lambda pages=p, hd=64, group=2, layers=1, stride=1 << 20: L.unimp_kv4_reorder_beams(pages, stride, layers, 4, 2, hd, p, 3, group, 2, p, p, None)
     assert b(pages=None) == ARG and b(hd=65) == b(group=17) == b(layers=1 << 17) == SHAPE and b(pages=odd) == b(stride=(1 << 20) + 4) == ALIGN and b(group=1) == 0
 

@@ -373,3 +373,86 @@ def test_hidden_pages(ops):
     got = ops.kv4_attn_decode(q.cuda(), pages.cuda(), tables.cuda(), lens.cuda(), 0.125)
     check(got, want, bound)
     assert not got[1].any()
+
+
+def test_lengths_beyond_the_table_and_odd_views(ops):
+    """a length above 32 x width stands for the whole table, a negative one for nothing; q and k / v views that no 16-byte load can read are copied; out may be q"""
+    hd, kvh, W = 64, 2, 3
+    pages, tables = paged(3, W, kvh, hd, seed=71)
+    lens = torch.tensor([1000, -4, 2 ** 31 - 1], dtype=torch.int32)
+    q = rnd(3, kvh, hd, seed=72)
+    want, bound = R.attend(q, pages, tables, torch.tensor([96, 0, 96]), 0.125)
+    raw = torch.zeros(3, kvh, hd + 3, dtype=bf16, device="cuda")
+    raw[..., 1:hd + 1] = q.cuda()
+    p, t, n = pages.cuda(), tables.cuda(), lens.cuda()
+    check(ops.kv4_attn_decode(raw[..., 1:hd + 1], p, t, n, 0.125), want, bound)
+    own = q.cuda()
+    check(ops.kv4_attn_decode(own, p, t, n, 0.125, out=own), want, bound)
+    k = rnd(40, kvh, hd + 1, seed=73).cuda()
+    ops.kv4_write(k[..., 1:], k[..., :hd], p, torch.arange(40, device="cuda"))
+    gk, gv = ops.kv4_read(p, torch.arange(40, device="cuda"), hd)
+    assert torch.equal(gk.cpu().double(), R.held(k[..., 1:].cpu())) and torch.equal(gv.cpu().double(), R.held(k[..., :hd].cpu()))
+
+
+def test_nothing_to_do(ops):
+    """no rows, no tokens, no columns"""
+    e = lambda *s, dt=bf16: torch.empty(s, dtype=dt, device="cuda")
+    pages = torch.zeros((2, 3, R.page_bytes(80)), dtype=torch.uint8, device="cuda")
+    assert ops.kv4_attn_decode(e(0, 3, 80), pages, e(0, 4, dt=torch.int32), e(0, dt=torch.int32), 1.0).shape == (0, 3, 80)
+    q = rnd(2, 6, 80).cuda()
+    assert not ops.kv4_attn_decode(q, pages, e(2, 0, dt=torch.int32), torch.tensor([5, 0], dtype=torch.int32, device="cuda"), 1.0).any()
+    ops.kv4_write(e(0, 3, 80), e(0, 3, 80), pages, e(0, dt=torch.int64))
+    assert ops.kv4_read(pages, e(0, dt=torch.int64), 80)[0].shape == (0, 3, 80)
+    assert ops.kv4_rope_append(e(0, 720), 3, 240, 80, (0, 80, 160), 0, None, None, pages, e(0, dt=torch.int64)).shape == (0, 3, 80)
+    assert not pages.any()
+
+
+def test_a_pool_beyond_32_bits(ops):
+    """pages at byte offsets above 4 GiB: written, appended to, read, attended to, moved"""
+    hd, kvh, n_pages = 128, 4, 300_000                              # 5.2 GB
+    pool = torch.zeros((n_pages, kvh, R.page_bytes(hd)), dtype=torch.uint8, device="cuda")
+    ids = torch.tensor([[n_pages - 1, 5, n_pages - 70], [n_pages - 2, 5, n_pages - 71]], dtype=torch.int32)
+    t = torch.arange(70)
+    slots = torch.cat([ids[r].long()[t // 32] * 32 + t % 32 for r in range(2)])
+    kv = rnd(2, 140, kvh, hd, seed=81)
+    ops.kv4_write(kv[0].cuda(), kv[1].cuda(), pool, slots.cuda())
+    qkv = rnd(2, 3 * kvh * hd, seed=82)
+    ops.kv4_rope_append(qkv.cuda(), kvh, hd, hd, (0, kvh * hd, 2 * kvh * hd), 0, None, None, pool, (ids[:, 2].long() * 32 + 6).cuda())
+    small = pool[ids.view(-1).long()].cpu()                         # what the two rows name, as a pool of six pages
+    q = rnd(2, kvh, hd, seed=83)
+    lens = torch.tensor([71, 71], dtype=torch.int32)
+    want, bound = R.attend(q, small, torch.arange(6, dtype=torch.int32).view(2, 3), lens, 0.1)
+    check(ops.kv4_attn_decode(q.cuda(), pool, ids.cuda(), lens.cuda(), 0.1), want, bound)
+    k, v = R.unpack(small, hd)
+    assert torch.equal(k[2, :, 6], R.held(qkv.view(2, 3, kvh, hd)[0, 1])) and torch.equal(v[5, :, 6], R.held(qkv.view(2, 3, kvh, hd)[1, 2]))
+    gk, _ = ops.kv4_read(pool, slots[:32].cuda(), hd)
+    assert torch.equal(gk.cpu().double(), R.held(kv[0, :32]))
+    tab = ids.cuda()
+    ops.kv4_reorder_beams(pool, tab, 2, torch.tensor([1, 1], device="cuda"), torch.tensor([71, 71], device="cuda"))
+    assert tab.tolist() == [[n_pages - 2, 5, n_pages - 70], [n_pages - 2, 5, n_pages - 71]] and torch.equal(pool[n_pages - 70], pool[n_pages - 71])
+    del pool
+    torch.cuda.empty_cache()
+
+
+def test_two_streams_at_once(ops):
+    """the same pool read by calls on two streams, each with partials of its own, while a third writes other pages"""
+    hd, kvh, rows, W = 80, 4, 8, 70
+    pages, tables = paged(rows, W, kvh, hd, seed=91, extra=40)
+    free = sorted(set(range(pages.shape[0])) - set(tables.view(-1).tolist()))
+    p, t = pages.cuda(), tables.cuda()
+    lens = torch.full((rows,), W * 32 - 5, dtype=torch.int32, device="cuda")
+    qs = [rnd(rows, kvh, hd, seed=92 + i).cuda() for i in range(2)]
+    want = [ops.kv4_attn_decode(q, p, t, lens, 0.11) for q in qs]
+    k = rnd(32 * len(free), kvh, hd, seed=95).cuda()
+    slots = (torch.tensor(free)[:, None] * 32 + torch.arange(32)).view(-1).cuda()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.kv4_attn_decode(qs[i], p, t, lens, 0.11))
+        with torch.cuda.stream(streams[2]):
+            ops.kv4_write(k, k, p, slots)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])

@@ -174,8 +174,8 @@ __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restric
 
 extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, void* pages, int64_t n_pages, int heads,
                                int hd, const int64_t* slots, int64_t tokens, void* stream) {
-  if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
   if (tokens <= 0 || heads <= 0 || n_pages <= 0) return UNIMP_OK;
+  if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
   if (heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^31 token heads");
   if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
@@ -267,8 +267,8 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
 
 extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,
                                      const float* cos_rows, const float* sin_rows, void* q_out, void* pages, int64_t n_pages, const int64_t* slots, void* stream) {
-  if (!qkv || !q_out || !pages || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
   if (rows <= 0 || heads <= 0) return UNIMP_OK;
+  if (!qkv || !q_out || !pages || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
   if (rot < 0 || (rot & 1) || rot > hd || rows > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_rope_append: rot even and at most the head dim, at most 65535 rows");
   if (((uintptr_t)pages & 15) || ((uintptr_t)q_out & 3)) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_rope_append: 16-byte aligned pages, 4-byte aligned q_out");
   return kv4_for_hd(hd, [&](auto d) {
@@ -352,8 +352,8 @@ __global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restr
 
 extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, const int64_t* slots, int64_t tokens, void* k,
                               void* v, void* stream) {
-  if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
+  if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
   if (layers > 65535 || heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23)
     return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^31 token heads");
@@ -462,8 +462,8 @@ extern "C" int unimp_page_tables_extend(int32_t* tables, int rows, int width, co
                                         int32_t* cursor_out, int64_t* slots, int64_t max_tokens, int32_t* cu, void* stream) {
   if (!tables || !mapped || !cached || !fresh || !free_pages || !cursor || !mapped_out || !cursor_out || !cu || (max_tokens > 0 && !slots))
     return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: null pointer");
-  if (rows <= 0 || width <= 0 || n_free < 0 || max_tokens < 0 || group < 1 || (rows % group))
-    return unimp_set_error(UNIMP_ERR_SHAPE, "page_tables_extend: rows a positive multiple of group, width positive");
+  if (rows <= 0 || rows > 65536 || width <= 0 || n_free < 0 || max_tokens < 0 || group < 1 || (rows % group))      // every workgroup sums over the rows before it
+    return unimp_set_error(UNIMP_ERR_SHAPE, "page_tables_extend: rows a positive multiple of group, at most 65536; width positive");
   if (mapped == mapped_out || cursor == cursor_out) return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: the blocks read mapped and cursor throughout; outputs of their own");
   PageArgs a{tables, mapped, cached, fresh, cover, free_pages, cursor, shared_len, mapped_out, cursor_out, cu, slots, (long)max_tokens, rows, width, n_free, group};
   // a workgroup per row below 1 024 rows (600 rows x 300 tokens: 5.1 us against 6.3 for a wave per row; 2 000 x 1: 8.9 against 6.2, 4 000 x 2: 17.9 against 10.0)

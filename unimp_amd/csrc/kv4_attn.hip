@@ -418,7 +418,8 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   return p;
 }
 static int kv4_attn_check(const unimp_kv4_attn_desc* d) {
-  if (!d || !d->q || !d->pages || !d->tables || !d->lens || !d->out) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: null pointer");
+  if (d && (d->rows == 0 || d->heads == 0)) return UNIMP_OK;                        // empty tensors have no pointers
+  if (!d || !d->q || !d->pages || (!d->tables && d->width) || !d->lens || !d->out) return unimp_set_error(UNIMP_ERR_ARG, "kv4_attn_decode: null pointer");
   if (d->kv_heads <= 0 || d->heads < 0 || d->heads % d->kv_heads || d->heads / d->kv_heads > 16 || d->width < 0 || d->width > 64 * 4 * KV4_MAX_SLOTS || d->rows < 0 || d->rows > 32767 ||
       d->heads > 65535 || d->n_pages <= 0)
     return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_attn_decode: query heads a multiple of the key heads, at most 16 to one; at most 32767 rows, 65536 pages of a row; a pool with pages");
