@@ -1096,15 +1096,22 @@ def _kv4_refuse(what, rule, **args):
     raise ValueError(f"{what}: {rule}; got " + ", ".join(f"{k} = {say(v)}" for k, v in args.items()))
 
 
-def _kv4_launch(fn, what, tensors, args):
+def _kv4_launch(fn, tensors, args):
     """the launch on the current stream, if every tensor lives on the current HIP device (its stream would not order the call otherwise)"""
     dev = _current_device() if tensors[0].is_cuda else -1
     for t in tensors:
         if t is not None and t.get_device() != dev or dev < 0:
-            raise _lib.UnimpHipError(f"{what}: every tensor on the current HIP device ({'none' if dev < 0 else f'cuda:{dev}'}), got {t.device}")
-    rc = fn(*args, _raw_stream(dev) if _raw_stream is not None else _stream())
+            raise _lib.UnimpHipError(f"{fn}: every tensor on the current HIP device ({'none' if dev < 0 else f'cuda:{dev}'}), got {t.device}")
+    rc = (_KV4_FN.get(fn) or _kv4_fn(fn))(*args, _raw_stream(dev) if _raw_stream is not None else _stream())
     if rc:
-        check(rc, what)
+        check(rc, fn)
+
+
+_KV4_FN = {}
+
+
+def _kv4_fn(name):
+    return _KV4_FN.setdefault(name, getattr(_lib.lib(), "unimp_" + name))
 
 
 def _kv4_rows(t):
@@ -1116,24 +1123,25 @@ def _kv4_rows(t):
 def kv4_write(k, v, pages, slots):
     """quantise k and v [tokens, heads, hd] (bf16 views, e.g. a prefill's rotated keys) into the slots [tokens] (int64; slot s = token s % 32 of page s // 32; a slot
     outside the pool: the token is not written) of one layer's pages [n_pages, heads, kv4_page_bytes(hd)]."""
-    if not (k.dim() == 3 and k.shape == v.shape and k.dtype is bf16 and v.dtype is bf16 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous()
-            and pages.shape[2] == _KV4_BYTES.get(k.shape[2]) and pages.shape[1] == k.shape[1] and slots.dtype is _i64 and slots.dim() == 1
-            and slots.shape[0] == k.shape[0] and slots.is_contiguous()):
+    shape, pool = k.shape, pages.shape
+    if not (len(shape) == 3 and shape == v.shape and k.dtype is bf16 and v.dtype is bf16 and len(pool) == 3 and pages.dtype is _u8 and pages.is_contiguous()
+            and pool[1] == shape[1] and pool[2] == _KV4_BYTES.get(shape[2]) and slots.dtype is _i64 and slots.shape == shape[:1] and slots.is_contiguous()):
         _kv4_refuse("kv4_write", "k, v bf16 [tokens, heads, hd]; pages contiguous uint8 [n_pages, heads, kv4_page_bytes(hd)]; slots contiguous int64 [tokens]", k=k, v=v, pages=pages,
                     slots=slots)
     k, v = _kv4_rows(k), _kv4_rows(v)
     (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    _kv4_launch(_lib.lib().unimp_kv4_write, "kv4_write", (pages, k, v, slots), (k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, pages.data_ptr(), pages.shape[0], k.shape[1],
-                                                                                k.shape[2], slots.data_ptr(), k.shape[0]))
+    _kv4_launch("kv4_write", (pages, k, v, slots), (k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, pages.data_ptr(), pool[0], shape[1], shape[2], slots.data_ptr(), shape[0]))
 
 
 def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows, pages, slots):
     """decode step on the 4-bit cache: rotate q and k of every row (row r with ITS table row cos_rows / sin_rows [rows, rot // 2]; rot = 0: none), quantise the
     rotated k and v into slot slots[r] of one layer's pages, return the rotated q [rows, heads, hd].  Operand layout of decode_rope_append; qkv2d is left unrotated."""
     rows, width = qkv2d.shape
+    stride, unit = qkv2d.stride()
     q_off, k_off, v_off = offs
-    if not (qkv2d.dtype is bf16 and qkv2d.stride(1) == 1 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous() and pages.shape[1] == heads
-            and pages.shape[2] == _KV4_BYTES.get(hd) and min(q_off, k_off, v_off, head_stride) >= 0 and max(q_off, k_off, v_off) + (heads - 1) * head_stride + hd <= width
+    pool = pages.shape
+    if not (qkv2d.dtype is bf16 and unit == 1 and len(pool) == 3 and pages.dtype is _u8 and pages.is_contiguous() and pool[1] == heads
+            and pool[2] == _KV4_BYTES.get(hd) and min(q_off, k_off, v_off, head_stride) >= 0 and max(q_off, k_off, v_off) + (heads - 1) * head_stride + hd <= width
             and slots.dtype is _i64 and slots.shape == (rows,) and slots.is_contiguous()
             and (rot == 0 or (0 < rot <= hd and not rot & 1 and cos_rows.dtype is _f32 and sin_rows.dtype is _f32 and cos_rows.shape == (rows, rot // 2) == sin_rows.shape
                               and cos_rows.is_contiguous() and sin_rows.is_contiguous()))):
@@ -1141,9 +1149,9 @@ def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows
                     "rot even, at most hd; cos, sin contiguous fp32 [rows, rot // 2]", qkv=qkv2d, heads=heads, head_stride=head_stride, hd=hd, offs=offs, rot=rot, cos=cos_rows,
                     sin=sin_rows, pages=pages, slots=slots)
     q = qkv2d.new_empty((rows, heads, hd))
-    _kv4_launch(_lib.lib().unimp_kv4_rope_append, "kv4_rope_append", (pages, qkv2d, slots) + ((cos_rows, sin_rows) if rot else ()),
-                (qkv2d.data_ptr(), qkv2d.stride(0), head_stride, rows, heads, hd, q_off, k_off, v_off, rot, cos_rows.data_ptr() if rot else None,
-                 sin_rows.data_ptr() if rot else None, q.data_ptr(), pages.data_ptr(), pages.shape[0], slots.data_ptr()))
+    _kv4_launch("kv4_rope_append", (pages, qkv2d, slots, cos_rows, sin_rows) if rot else (pages, qkv2d, slots),
+                (qkv2d.data_ptr(), stride, head_stride, rows, heads, hd, q_off, k_off, v_off, rot, cos_rows.data_ptr() if rot else None,
+                 sin_rows.data_ptr() if rot else None, q.data_ptr(), pages.data_ptr(), pool[0], slots.data_ptr()))
     return q
 
 
@@ -1161,13 +1169,13 @@ def kv4_read(pages, slots, hd):
     """the values held in slots [tokens] (int64; outside the pool: zeros) of pages [(layers,) n_pages, heads, kv4_page_bytes(hd)] -> k, v bf16
     [(layers,) tokens, heads, hd]: exactly what the attention multiplies"""
     layers, stride = _kv4_layers(pages)
-    if not (layers and pages.shape[-1] == _KV4_BYTES.get(hd) and slots.dtype is _i64 and slots.dim() == 1 and slots.is_contiguous()):
+    pool, tokens = pages.shape, slots.numel()
+    if not (layers and pool[-1] == _KV4_BYTES.get(hd) and slots.dtype is _i64 and slots.dim() == 1 and slots.is_contiguous()):
         _kv4_refuse("kv4_read", "pages uint8 [(layers,) n_pages, heads, kv4_page_bytes(hd)], every layer contiguous; slots contiguous int64 [tokens]", pages=pages, slots=slots, hd=hd)
-    tokens, (n_pages, heads) = slots.shape[0], pages.shape[-3:-1]
-    shape = (*pages.shape[:-3], tokens, heads, hd)
-    k = pages.new_empty(shape, dtype=bf16)
+    n_pages, heads = pool[-3], pool[-2]
+    k = pages.new_empty((tokens, heads, hd) if len(pool) == 3 else (layers, tokens, heads, hd), dtype=bf16)
     v = torch.empty_like(k)
-    _kv4_launch(_lib.lib().unimp_kv4_read, "kv4_read", (pages, slots), (pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr()))
+    _kv4_launch("kv4_read", (pages, slots), (pages.data_ptr(), stride, layers, n_pages, heads, hd, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr()))
     return k, v
 
 
@@ -1179,18 +1187,19 @@ def page_tables_extend(tables, mapped, cached, new, free_pages, cursor, max_toke
     Returns (mapped, cursor, slots, cu): the new column counts and free-list position (above n: pages were missing, their columns are -1), slots int64 [max_tokens] of
     the new tokens in packed order (-1: none) and int32 [rows + 1] the packed index of every row's first new token."""
     rows, width = tables.shape
+    row = mapped.shape
     if not (tables.dtype is _i32 and tables.is_contiguous() and rows * width > 0 and group >= 1 and rows % group == 0 and max_tokens >= 0
-            and mapped.dtype is _i32 and mapped.shape == (rows,) and mapped.is_contiguous() and cached.dtype is _i32 and cached.shape == (rows,) and cached.is_contiguous()
-            and new.dtype is _i32 and new.shape == (rows,) and new.is_contiguous() and cursor.dtype is _i32 and cursor.shape == (1,)
+            and row == (rows,) and row == cached.shape and row == new.shape and mapped.dtype is _i32 and cached.dtype is _i32 and new.dtype is _i32 and mapped.is_contiguous()
+            and cached.is_contiguous() and new.is_contiguous() and cursor.dtype is _i32 and cursor.shape == (1,)
             and free_pages.dtype is _i32 and free_pages.dim() == 1 and free_pages.is_contiguous()
-            and (cover is None or (cover.dtype is _i32 and cover.shape == (rows,) and cover.is_contiguous()))
+            and (cover is None or (cover.dtype is _i32 and cover.shape == row and cover.is_contiguous()))
             and (shared_len is None or (shared_len.dtype is _i32 and shared_len.shape == (rows // group,) and shared_len.is_contiguous()))):
         _kv4_refuse("page_tables_extend", "contiguous int32: tables [rows, width], mapped, cached, new, cover [rows], free_pages [n], cursor [1], shared_len [rows // group]; rows a multiple "
                     "of group", tables=tables, mapped=mapped, cached=cached, new=new, cover=cover, free_pages=free_pages, cursor=cursor, group=group, shared_len=shared_len,
                     max_tokens=max_tokens)
     ints, slots = tables.new_empty(2 * rows + 2), tables.new_empty(max_tokens, dtype=_i64)
     p = ints.data_ptr()                                       # mapped [rows], cursor [1], cu [rows + 1]
-    _kv4_launch(_lib.lib().unimp_page_tables_extend, "page_tables_extend", (tables, mapped, cached, new, free_pages, cursor, cover, shared_len),
+    _kv4_launch("page_tables_extend", (tables, mapped, cached, new, free_pages, cursor, cover, shared_len),
                 (tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), None if cover is None else cover.data_ptr(), free_pages.data_ptr(),
                  free_pages.shape[0], cursor.data_ptr(), group, None if shared_len is None else shared_len.data_ptr(), p, p + 4 * rows, slots.data_ptr(), max_tokens, p + 4 * rows + 4))
     mapped_out, cursor_out, cu = ints.split((rows, 1, rows + 1))
@@ -1203,13 +1212,14 @@ def kv4_reorder_beams(pages, tables, group, src_local, pos):
     filled is copied in pages [(layers,) n_pages, heads, page bytes] into the row's own."""
     layers, stride = _kv4_layers(pages)
     rows, width = tables.shape
-    hd = _KV4_HD.get(pages.shape[-1], 0)
+    pool = pages.shape
+    hd = _KV4_HD.get(pool[-1], 0)
     if not (layers and hd and tables.dtype is _i32 and tables.is_contiguous() and 1 <= group <= 16 and rows % group == 0 and src_local.dtype is _i64 and pos.dtype is _i64
             and src_local.shape == (rows,) == pos.shape and src_local.is_contiguous() and pos.is_contiguous()):
         _kv4_refuse("kv4_reorder_beams", "pages uint8 [(layers,) n_pages, heads, page bytes], every layer contiguous; tables contiguous int32 [rows, width], rows a multiple of group (at most "
                     "16); src_local, pos contiguous int64 [rows]", pages=pages, tables=tables, group=group, src_local=src_local, pos=pos)
-    _kv4_launch(_lib.lib().unimp_kv4_reorder_beams, "kv4_reorder_beams", (pages, tables, src_local, pos),
-                (pages.data_ptr(), stride, layers, pages.shape[-3], pages.shape[-2], hd, tables.data_ptr(), width, group, rows // group, src_local.data_ptr(), pos.data_ptr()))
+    _kv4_launch("kv4_reorder_beams", (pages, tables, src_local, pos),
+                (pages.data_ptr(), stride, layers, pool[-3], pool[-2], hd, tables.data_ptr(), width, group, rows // group, src_local.data_ptr(), pos.data_ptr()))
 
 
 _KV4_ATTN = struct.Struct("@PqqPqiiPqiPiifPPqqiP")              # unimp_kv4_attn_desc (tests/test_kv4_cpu.py compares it with the ctypes mirror)
@@ -1231,26 +1241,33 @@ def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_l
     tables [rows, width] (int32) name in one layer's pool [n_pages, kv heads, page bytes]; heads a multiple of kv heads, at most 16 to one.  alibi: fp32 [heads] slopes.  A
     row of length 0 gives zeros; a page id outside the pool hides its tokens.  group > 1 with shared_len (int32 [rows // group]): the rows of a group (the beams of a
     prompt) name the same pages below shared_len // 32 columns; those are read once per group.  Returns o [rows, heads, hd]."""
-    if out is None:
-        out = q.new_empty(q.shape)
+    shape, pool, table = q.shape, pages.shape, tables.shape
     grouped = group > 1 and shared_len is not None
-    if not (q.dim() == 3 and q.dtype is bf16 and pages.dim() == 3 and pages.dtype is _u8 and pages.is_contiguous() and pages.shape[2] == _KV4_BYTES.get(q.shape[2])
-            and pages.shape[0] > 0 and pages.shape[1] > 0 and q.shape[1] % pages.shape[1] == 0 and q.shape[1] <= 16 * pages.shape[1]
-            and tables.dim() == 2 and tables.dtype is _i32 and tables.shape[0] == q.shape[0] and tables.stride(1) == 1
-            and lens.dtype is _i32 and lens.shape == (q.shape[0],) and lens.is_contiguous()
-            and (alibi is None or (alibi.dtype is _f32 and alibi.shape == (q.shape[1],) and alibi.is_contiguous()))
-            and (shared_len is None or (group >= 1 and q.shape[0] % group == 0 and shared_len.dtype is _i32 and shared_len.shape == (q.shape[0] // group,) and shared_len.is_contiguous()))
-            and out.dtype is bf16 and out.shape == q.shape and out.stride(2) == 1):
+    if not (len(shape) == 3 and q.dtype is bf16 and len(pool) == 3 and pages.dtype is _u8 and pages.is_contiguous() and pool[2] == _KV4_BYTES.get(shape[2])
+            and pool[0] > 0 and pool[1] > 0 and shape[1] % pool[1] == 0 and shape[1] <= 16 * pool[1]
+            and len(table) == 2 and tables.dtype is _i32 and table[0] == shape[0] and tables.stride(1) == 1
+            and lens.dtype is _i32 and lens.shape == shape[:1] and lens.is_contiguous()
+            and (alibi is None or (alibi.dtype is _f32 and alibi.shape == shape[1:2] and alibi.is_contiguous()))
+            and (shared_len is None or (group >= 1 and shape[0] % group == 0 and shared_len.dtype is _i32 and shared_len.shape == (shape[0] // group,) and shared_len.is_contiguous()))
+            and (out is None or (out.dtype is bf16 and out.shape == shape and out.stride(2) == 1))):
         _kv4_refuse("kv4_attn_decode", "q and out bf16 [rows, heads, hd]; pages contiguous uint8 [n_pages, kv heads, kv4_page_bytes(hd)], heads a multiple of kv heads, at most 16 to one; "
                     "tables int32 [rows, width] with unit column stride; lens contiguous int32 [rows]; alibi contiguous fp32 [heads]; shared_len contiguous int32 [rows // group]",
                     q=q, pages=pages, tables=tables, lens=lens, alibi=alibi, group=group, shared_len=shared_len, out=out)
-    q = _kv4_rows(q)
-    (rows, heads, hd), (qr, qh, _), (o_r, o_h, _) = q.shape, q.stride(), out.stride()
-    n_pages, kv_heads, _ = pages.shape
-    width = tables.shape[1]
+    rows, heads, hd = shape
+    qr, qh, unit = q.stride()
+    if unit != 1 or qr & 7 or qh & 7 or q.data_ptr() & 15:                            # no 16-byte loads from this view
+        q = q.contiguous()
+        qr, qh, _ = q.stride()
+    if out is None:
+        out = q.new_empty(shape)
+        o_r, o_h = heads * hd, hd
+    else:
+        o_r, o_h, _ = out.stride()
+    n_pages, kv_heads, _ = pool
+    width = table[1]
     n = _kv4_workspace(rows, heads, kv_heads, hd, width, group if grouped else 1)
-    ws = q.new_empty(n, dtype=_f32) if n else None                   # of this call: nothing that two streams or graphs could share
+    ws = q.new_empty(n, dtype=_f32) if n else None            # of this call: nothing that two streams or graphs could share
     d = _KV4_ATTN.pack(q.data_ptr(), qr, qh, pages.data_ptr(), n_pages, kv_heads, hd, tables.data_ptr(), tables.stride(0), width, lens.data_ptr(), rows, heads, scale,
                        0 if alibi is None else alibi.data_ptr(), out.data_ptr(), o_r, o_h, group if grouped else 1, shared_len.data_ptr() if grouped else 0)
-    _kv4_launch(_lib.lib().unimp_kv4_attn_decode, "kv4_attn_decode", (q, pages, tables, lens, out, alibi, shared_len), (d, ws.data_ptr() if n else None))
+    _kv4_launch("kv4_attn_decode", (q, pages, tables, lens, out, alibi, shared_len), (d, ws.data_ptr() if n else None))
     return out
