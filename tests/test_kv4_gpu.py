@@ -230,7 +230,7 @@ def test_reorder_beams(ops, K, groups, heads, hd, layers):
 @pytest.mark.parametrize("rows,kvh,G,lens,alibi", [
     (1, 1, 1, [1], False), (5, 2, 1, [0, 1, 31, 32, 33], True), (3, 3, 2, [64, 7, 200], False), (2, 1, 16, [129, 300], True), (4, 2, 3, [96, 0, 1, 511], True),
     (2, 4, 8, [1500, 40], False), (1, 2, 1, [4500], True), (70, 16, 1, [5, 130, 64, 0, 513, 31, 200], False), (40, 32, 2, [77, 1, 90, 0], True),
-    (9, 2, 4, [3000, 0, 1777, 2111], True)])
+    (9, 2, 4, [3000, 0, 1777, 2111], True), (3, 2, 6, [700, 33, 0], True), (1, 1, 5, [2500], False), (2, 1, 9, [95, 400], True)])
 def test_attention(ops, hd, rows, kvh, G, lens, alibi):
     lens = (lens * rows)[:rows]
     W = (max(lens) + 31) // 32 + 1
@@ -272,7 +272,7 @@ def poison_behind(page, n, hd):
                                                           (128, 10, 1, 2, 4, 200, 90), (64, 2, 2, 2, 8, 1000, 33),
                                                           # from 8 192 pages of all rows and key heads on the shared pages are read once per group
                                                           (80, 10, 2, 32, 1, 400, 20), (64, 16, 2, 32, 1, 290, 40), (128, 2, 5, 32, 8, 930, 70), (128, 4, 3, 32, 4, 700, 30),
-                                                          (80, 3, 2, 16, 2, 2700, 40), (64, 5, 2, 16, 3, 1663, 3)])
+                                                          (80, 3, 2, 16, 2, 2700, 40), (64, 5, 2, 16, 3, 1663, 3), (80, 3, 4, 32, 5, 800, 40)])
 def test_attention_beam_groups(ops, hd, K, groups, kvh, G, prompt, more):
     """the beams of a prompt name its whole pages together; with and without room for all their queries in one tile; ragged lengths behind the prompt"""
     rows = K * groups

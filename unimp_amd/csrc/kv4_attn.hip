@@ -10,7 +10,9 @@
 //   o^T     += V^T P^T on v_mfma_f32_16x16x32_bf16: A = V's nibbles through v_cvt_scalef32_pk_bf16_fp4 (exact), B = p times the token's V scale, which differs per 32 dims.
 //            p is split in two bf16 (16 bits kept).  The scale blocks and the two halves are COLUMNS of B where the queries leave room: with one or two queries
 //            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
-//            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 2: 16 queries, block and half as products.
+//            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 3: (query, half) columns, a product per block;
+//            MODE 2: 16 queries, block and half as products.  Measured, 64 rows x 8 key heads x 128 dims of up to 8 000 tokens (all of 8 000), TB/s of pages: MODE 0 (1 or 2 queries
+//            of a key head) 5.0 (5.7), MODE 1 (4) 4.8 (5.5), MODE 3 (8) 4.2 (5.0; as MODE 2 it was 3.9 (4.6)), MODE 2 (16) 3.7 (4.3).
 // Bound by the bytes of the pages: 17 / 32 of a byte per element.
 #include <type_traits>
 #include "kv4.h"
@@ -29,7 +31,7 @@ struct Kv4AttnArgs {
 
 template <int D, int MODE> struct Kv4Cols {
   static constexpr int NBP = D == 64 ? 2 : 4;                                     // scale blocks as columns (three of head dim 80 in four)
-  static constexpr int VAR = MODE == 0 ? 2 * NBP : MODE == 1 ? NBP : 1, Q = 16 / VAR;
+  static constexpr int VAR = MODE == 0 ? 2 * NBP : MODE == 1 ? NBP : MODE == 3 ? 2 : 1, Q = 16 / VAR;
 };
 
 template <int D> struct Kv4Frag {        // one page as a wave holds it
@@ -258,6 +260,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
     } else {
+      if constexpr (MODE == 3) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hi[j] = var ? lo[j] : hi[j];
+      }
       auto block = [&](auto BLK) {                                                // four lanes hold the four blocks' scales: taken from the neighbour (quad_perm)
         constexpr int blk = decltype(BLK)::value;
         uint32_t d0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)vs0, blk * 0x55, 0xf, 0xf, true);
@@ -267,11 +273,15 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float s0 = vscale(j < 2 ? d0 : d1, 2 * j & 3), s1 = vscale(j < 2 ? d0 : d1, (2 * j + 1) & 3);
-          bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);
-          bl.d[j] = pack(lo[2 * j] * s0, lo[2 * j + 1] * s1);
+          bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);                     // MODE 3: hi is the half that this column holds
+          if constexpr (MODE == 2) bl.d[j] = pack(lo[2 * j] * s0, lo[2 * j + 1] * s1);
         }
 #pragma unroll
-        for (int i = 2 * blk; i < 2 * blk + 2; ++i) if (i < NI) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
+        for (int i = 2 * blk; i < 2 * blk + 2; ++i) if (i < NI) {
+          const bf16x8 v = value(i);
+          acc[i] = MFMA16(v, bh.v, acc[i]);
+          if constexpr (MODE == 2) acc[i] = MFMA16(v, bl.v, acc[i]);
+        }
       };
       block(std::integral_constant<int, 0>()); block(std::integral_constant<int, 1>());
       if constexpr (P::NB > 2) block(std::integral_constant<int, 2>());
@@ -293,11 +303,11 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     f32x4 x = acc[i];
-    if constexpr (MODE == 0) {
+    if constexpr (MODE == 0 || MODE == 3) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], 1, 64);                // the two halves of p
     }
-    const bool mine = MODE == 0 ? var == 2 * (i >> 1) : MODE == 1 ? var == (i >> 1) : true;
+    const bool mine = MODE == 0 ? var == 2 * (i >> 1) : MODE == 1 ? var == (i >> 1) : MODE == 3 ? var == 0 : true;
     if (mine && qi < nq) *(f32x4*)&so[w][qi][16 * i + 4 * g] = x;
   }
   if (var == 0 && g == 0) { sm[w][qi] = m; sl[w][qi] = l; }
@@ -390,14 +400,14 @@ struct Kv4Plan { int mode, nw, chunk, slots, group, chunk_p, slots_p; int64_t fl
 static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   Kv4Plan p;
   auto clamp = [](long x, long lo, long hi) { return (int)(x < lo ? lo : x > hi ? hi : x); };
-  auto mode = [&](int nq) { const int nbp = d->hd == 64 ? 2 : 4; return nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : 2; };
+  auto mode = [&](int nq) { const int nbp = d->hd == 64 ? 2 : 4; return nq <= 8 / nbp ? 0 : nq <= 16 / nbp ? 1 : nq <= 8 ? 3 : 2; };
   const int G = d->heads / d->kv_heads;
   const long units = (long)d->rows * d->kv_heads;
   p.mode = mode(G);
   // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads, pages = rows x heads x columns: 10 beams x 80, prompt
   // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
-  p.nw = p.mode == 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
+  p.nw = p.mode >= 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
   // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 66.7 us, 48 61.6, 64 67.4, 96 61.8)
   const int most = d->width <= 64 ? 64 : 48;
   p.chunk = clamp((long)d->width * units / 1024, units < 512 ? 4 * p.nw : most, most);
@@ -449,7 +459,7 @@ static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t 
   } while (0)
     if (p.mode == 0) KV4_G(0);
     else if (p.mode == 1) KV4_G(1);
-    else KV4_G(2);
+    else if constexpr (D > 64) KV4_G(3);                                         // a group's rows have at most 8 queries each
 #undef KV4_G
     kv4_merge_launch<D>(a, p, s);
     return;
@@ -467,7 +477,8 @@ static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t 
   } while (0)
   if (p.mode == 0) KV4_W(0);
   else if (p.mode == 1) KV4_W(1);
-  else KV4_L(2, 4);
+  else if (p.mode == 2) KV4_L(2, 4);
+  else if constexpr (D > 64) KV4_L(3, 4);                                         // 5 ... 8 queries; of head dim 64 they are MODE 1
 #undef KV4_W
 #undef KV4_L
   if (a.ws) kv4_merge_launch<D>(a, p, s);
