@@ -272,7 +272,8 @@ def poison_behind(page, n, hd):
                                                           (128, 10, 1, 2, 4, 200, 90), (64, 2, 2, 2, 8, 1000, 33),
                                                           # from 8 192 pages of all rows and key heads on the shared pages are read once per group
                                                           (80, 10, 2, 32, 1, 400, 20), (64, 16, 2, 32, 1, 290, 40), (128, 2, 5, 32, 8, 930, 70), (128, 4, 3, 32, 4, 700, 30),
-                                                          (80, 3, 2, 16, 2, 2700, 40), (64, 5, 2, 16, 3, 1663, 3), (80, 3, 4, 32, 5, 800, 40)])
+                                                          (80, 3, 2, 16, 2, 2700, 40), (64, 5, 2, 16, 3, 1663, 3), (80, 3, 4, 32, 5, 800, 40),
+                                                          (128, 2, 3, 32, 1, 1400, 20), (80, 4, 2, 32, 1, 1000, 80), (128, 2, 2, 32, 3, 2100, 20), (64, 2, 4, 32, 1, 1100, 10), (64, 5, 2, 32, 1, 860, 60)])
 def test_attention_beam_groups(ops, hd, K, groups, kvh, G, prompt, more):
     """the beams of a prompt name its whole pages together; with and without room for all their queries in one tile; ragged lengths behind the prompt"""
     rows = K * groups

@@ -340,10 +340,11 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 template <int D, int MODE, int NW, bool ALIBI>
 __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
 
-// beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once
-template <int D, int MODE, bool ALIBI>
+// beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once,
+// in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: 45.6 us, 49.0 as MODE 2)
+template <int D, int MODE, int GMODE, bool ALIBI>
 __global__ __launch_bounds__(256) void kv4_attn_group_kernel(Kv4AttnArgs a) {
-  if ((int)blockIdx.z >= (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) kv4_attn_part<D, 2, 4, 1, ALIBI, true>(a);
+  if ((int)blockIdx.z >= (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) kv4_attn_part<D, GMODE, 4, 1, ALIBI, true>(a);
   else kv4_attn_part<D, MODE, 1, KV4_TEAMS, ALIBI, false>(a);
 }
 
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(PARTS * D / 2) void kv4_attn_merge_kernel(Kv4AttnAr
   o[0] = f2bf(l == 0.f ? 0.f : o0 / l); o[1] = f2bf(l == 0.f ? 0.f : o1 / l);
 }
 
-struct Kv4Plan { int mode, nw, chunk, slots, group, chunk_p, slots_p; int64_t floats; };
+struct Kv4Plan { int mode, gmode, nw, chunk, slots, group, chunk_p, slots_p; int64_t floats; };
 static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   Kv4Plan p;
   auto clamp = [](long x, long lo, long hi) { return (int)(x < lo ? lo : x > hi ? hi : x); };
@@ -407,6 +408,7 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads, pages = rows x heads x columns: 10 beams x 80, prompt
   // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
+  p.gmode = mode(p.group * G);
   p.nw = p.mode >= 2 || p.group > 1 ? 4 : units <= 256 && d->width <= 32 ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
   // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 66.7 us, 48 61.6, 64 67.4, 96 61.8)
   const int most = d->width <= 64 ? 64 : 48;
@@ -452,14 +454,21 @@ template <int D>
 static void kv4_attn_launch(const Kv4AttnArgs& a, const Kv4Plan& p, hipStream_t s) {
   if (p.group > 1) {
     const dim3 grid(a.kv_heads, p.slots > p.slots_p ? p.slots : p.slots_p, (a.rows + KV4_TEAMS - 1) / KV4_TEAMS + a.rows / p.group);
-#define KV4_G(M)                                                                                             \
+#define KV4_G(M, GM)                                                                                         \
   do {                                                                                                       \
-    if (a.alibi) hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, true>), grid, dim3(256), 0, s, a);          \
-    else hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, false>), grid, dim3(256), 0, s, a);                 \
+    if (a.alibi) hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, GM, true>), grid, dim3(256), 0, s, a);      \
+    else hipLaunchKernelGGL((kv4_attn_group_kernel<D, M, GM, false>), grid, dim3(256), 0, s, a);             \
   } while (0)
-    if (p.mode == 0) KV4_G(0);
-    else if (p.mode == 1) KV4_G(1);
-    else if constexpr (D > 64) KV4_G(3);                                         // a group's rows have at most 8 queries each
+    // a row's own queries are at most half of the group's
+    if (p.gmode != 2) {
+      if constexpr (D == 64) { if (p.gmode == 0) KV4_G(0, 0); else KV4_G(0, 1); }
+      else if (p.gmode == 0) KV4_G(0, 0);
+      else if (p.gmode == 1) KV4_G(0, 1);
+      else if (p.mode == 0) KV4_G(0, 3);
+      else KV4_G(1, 3);
+    } else if (p.mode == 0) KV4_G(0, 2);
+    else if (p.mode == 1) KV4_G(1, 2);
+    else if constexpr (D > 64) KV4_G(3, 2);
 #undef KV4_G
     kv4_merge_launch<D>(a, p, s);
     return;
