@@ -448,11 +448,12 @@ int unimp_image_resize_normalize(const uint8_t* src, const unimp_image_desc* des
  * Slots and page ids outside the pool are never accessed: such a token is not written, reads as zero and is not attended to.  Pages need no initial contents. */
 int unimp_kv4_page_bytes(int hd);
 /* quantise k, v (bf16; element strides: token, head; unit dim stride) of `tokens` tokens into their slots.  Different tokens of one page may be written by different
- * calls or rows in any order; the same slot twice in one call holds one of the two. */
+ * calls or rows in any order; the slots >= 0 of one call are different (a slot named twice leaves unspecified
+ * contents in that token, in no other). */
 int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, void* pages, int64_t n_pages, int heads, int hd,
                     const int64_t* slots, int64_t tokens, void* stream);
 /* a decode step's tokens: rotate q and k of every row (half-split pairs, row r with ITS table row; rot = 0: none), write q (bf16, rounded once) to q_out
- * [rows][heads][hd] and quantise the rotated k and v into slot slots[r].  Operand layout of unimp_decode_rope_append; qkv is not modified.  The rotation is computed in
+ * [rows][heads][hd] and quantise the rotated k and v into slot slots[r] (different ones).  Operand layout of unimp_decode_rope_append; qkv is not modified.  The rotation is computed in
  * 64 bits from the fp32 tables. */
 int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,
                           const float* cos_rows, const float* sin_rows, void* q_out, void* pages, int64_t n_pages, const int64_t* slots, void* stream);

@@ -67,6 +67,7 @@ def test_python_refusals():
                                                      slots=s3), **kw})
     _bad("offset outside the row", lambda: app(offs=(0, 64, 192)))
     _bad("odd rot", lambda: app(rot=3))
+    _bad("no tables", lambda: app(rot=16))
     _bad("rot above the head dim", lambda: app(rot=66))
     _bad("tables of another shape", lambda: app(rot=64, cos_rows=torch.zeros(3, 16), sin_rows=torch.zeros(3, 16)))
     _bad("slots of another length", lambda: app(slots=s3[:2].contiguous()))

@@ -406,6 +406,45 @@ def test_nothing_to_do(ops):
     assert ops.kv4_read(pages, e(0, dt=torch.int64), 80)[0].shape == (0, 3, 80)
     assert ops.kv4_rope_append(e(0, 720), 3, 240, 80, (0, 80, 160), 0, None, None, pages, e(0, dt=torch.int64)).shape == (0, 3, 80)
     assert not pages.any()
+    # a pool of no pages: nothing is written, everything reads as zero; no free page is needed where none is taken
+    none, s2 = pages[:0], torch.tensor([3, -1], device="cuda")
+    ops.kv4_write(rnd(2, 3, 80).cuda(), rnd(2, 3, 80).cuda(), none, s2)
+    assert not ops.kv4_read(none, s2, 80)[0].any()
+    qkv = rnd(2, 720).cuda()
+    assert torch.equal(ops.kv4_rope_append(qkv, 3, 240, 80, (0, 80, 160), 0, None, None, none, s2), qkv.view(2, 3, 240)[..., :80])
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    tab = i32(7, 9, 4, -1).view(2, 2)
+    m, c, s, cu = ops.page_tables_extend(tab, i32(2, 1), i32(40, 1), i32(2, 3), e(0, dt=torch.int32), i32(11), 6)
+    assert (tab.tolist(), m.tolist(), c.item(), s.tolist(), cu.tolist()) == ([[7, 9], [4, -1]], [2, 1], 11, [296, 297, 129, 130, 131, -1], [0, 2, 5])
+    ops.kv4_reorder_beams(pages, e(0, 4, dt=torch.int32), 2, e(0, dt=torch.int64), e(0, dt=torch.int64))
+    ops.kv4_reorder_beams(pages, e(2, 0, dt=torch.int32), 2, torch.ones(2, dtype=torch.long, device="cuda"), torch.full((2,), 40, device="cuda"))
+
+
+def test_sums_beyond_32_bits(ops):
+    """lengths whose sums pass 32 bits: the counts stay at the largest value, no slot is written behind the room"""
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    big = 2 ** 31 - 1
+    tab = torch.full((3, 2), -1, dtype=torch.int32, device="cuda")
+    m, c, s, cu = ops.page_tables_extend(tab, i32(0, 0, 0), i32(0, 0, 5), i32(big, big, big), i32(8, 3), i32(big - 1), 70)
+    assert tab.tolist() == [[-1, -1]] * 3 and m.tolist() == [2, 2, 2] and c.item() == big and cu.tolist() == [0, big, big, big] and s.tolist() == [-1] * 70
+
+
+def test_one_row_of_a_misaligned_buffer(ops):
+    """views that count as contiguous and yet start at an odd element, or have one row and an odd row stride"""
+    hd, kvh = 64, 2
+    pages, tables = paged(1, 2, kvh, hd, seed=75)
+    n = torch.tensor([50], dtype=torch.int32)
+    q = rnd(1, kvh, hd, seed=76)
+    want, bound = R.attend(q, pages, tables, n, 0.125)
+    flat = torch.zeros(1 + kvh * hd, dtype=bf16, device="cuda")
+    flat[1:] = q.cuda().view(-1)
+    wide = torch.zeros(1, kvh * hd + 3, dtype=bf16, device="cuda")
+    wide[:, :kvh * hd] = q.cuda().view(1, -1)
+    p, slot = pages.cuda(), torch.tensor([int(tables[0, 1]) * 32 + 31], device="cuda")
+    for view in (flat[1:].view(1, kvh, hd), wide[:, :kvh * hd].view(1, kvh, hd)):
+        check(ops.kv4_attn_decode(view, p, tables.cuda(), n.cuda(), 0.125), want, bound)
+        ops.kv4_write(view, view, p, slot)
+        assert torch.equal(ops.kv4_read(p, slot, hd)[1].cpu().double(), R.held(q))
 
 
 def test_a_pool_beyond_32_bits(ops):

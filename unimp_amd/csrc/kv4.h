@@ -15,24 +15,19 @@
 
 #define KV4_PAGE 32
 
+__device__ __forceinline__ int kv4_nibble(int t) { return 4 * (t >> 4) + (t & 3); }      // token's nibble in its V dword
+
 template <int D> struct Kv4 {
   static constexpr int NB = (D + 31) / 32, NI = D / 16, VOFF = 16 * D, KS = 32 * D, VS = 32 * D + 32 * NB, BYTES = 32 * D + 64 * NB;
   static constexpr int BLK_LAST = D - 32 * (NB - 1);                              // dims of the last block: 32 or 16
   static __device__ __forceinline__ int k_byte(int t, int b) { return 512 * b + t * (b == NB - 1 ? BLK_LAST / 2 : 16); }   // first byte of (token, block)
   static __device__ __forceinline__ int v_dword(int t, int d) { return VOFF + 4 * (((t >> 2) & 3) * D + (d & 15) * NI + (d >> 4)); }
   static __device__ __forceinline__ int ks_byte(int t, int b) { return KS + 32 * b + 2 * (t & 15) + (t >> 4); }
-  static __device__ __forceinline__ int vs_byte(int t, int b) { return VS + 8 * NB * ((t >> 2) & 3) + 8 * b + kv4_nib(t); }
-  static __device__ __forceinline__ int kv4_nib(int t) { return 4 * (t >> 4) + (t & 3); }
+  static __device__ __forceinline__ int vs_byte(int t, int b) { return VS + 8 * NB * ((t >> 2) & 3) + 8 * b + kv4_nibble(t); }
 };
-__device__ __forceinline__ int kv4_nibble(int t) { return 4 * (t >> 4) + (t & 3); }      // token's nibble in its V dword
 
 // 2^(byte - 127); byte 255 (a block that held an infinity or a NaN): NaN.  Bytes written here are 2 ... 252 or 255.
 __device__ __forceinline__ float kv4_scale(uint32_t byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23); }
 // block exponent from the exponent field of the block's largest magnitude (floor(log2 amax) + 127; 255: not finite): E8M0 byte, at least 2 so that no held
 // value is subnormal
 __device__ __forceinline__ int kv4_scale_byte(int eb) { return eb == 255 ? 255 : max(eb - 2, 2); }
-__device__ __forceinline__ float kv4_value(uint32_t code) {                              // e2m1
-  const uint32_t m = code & 7u;
-  const float v = m < 4u ? 0.5f * (float)m : (m < 6u ? (float)m - 2.f : 2.f * (float)m - 8.f);
-  return (code & 8u) ? -v : v;
-}

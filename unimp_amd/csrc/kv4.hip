@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
 extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,
                                      const float* cos_rows, const float* sin_rows, void* q_out, void* pages, int64_t n_pages, const int64_t* slots, void* stream) {
   if (rows <= 0 || heads <= 0) return UNIMP_OK;
-  if (!qkv || !q_out || !pages || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
+  if (!qkv || !q_out || (!pages && n_pages > 0) || !slots || (rot && (!cos_rows || !sin_rows))) return unimp_set_error(UNIMP_ERR_ARG, "kv4_rope_append: null pointer");
   if (rot < 0 || (rot & 1) || rot > hd || rows > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_rope_append: rot even and at most the head dim, at most 65535 rows");
   if (((uintptr_t)pages & 15) || ((uintptr_t)q_out & 3)) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_rope_append: 16-byte aligned pages, 4-byte aligned q_out");
   return kv4_for_hd(hd, [&](auto d) {
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restr
 extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, const int64_t* slots, int64_t tokens, void* k,
                               void* v, void* stream) {
   if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
-  if (!pages || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
+  if ((!pages && n_pages > 0) || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
   if (layers > 65535 || heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23)
     return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^31 token heads");
@@ -450,9 +450,10 @@ __global__ __launch_bounds__(RPB == 1 ? 256 : 512) void page_tables_extend_kerne
   }
   if (blockIdx.y) return;
   for (int c = map + at; c < p.need; c += STEP) row[c] = lookup(c);
-  if (at == 0) { a.mapped_out[r] = max(map, p.need); a.cu[r] = (int)tok; }
+  auto to32 = [](long x) { return (int)min(x, 0x7fffffffl); };       // sums of nonsense lengths stay above every limit
+  if (at == 0) { a.mapped_out[r] = max(map, p.need); a.cu[r] = to32(tok); }
   if (r == a.rows - 1) {
-    if (at == 0) { a.cu[a.rows] = (int)(tok + n); a.cursor_out[0] = (int)(before + max(p.need - p.begin, 0)); }
+    if (at == 0) { a.cu[a.rows] = to32(tok + n); a.cursor_out[0] = to32(before + max(p.need - p.begin, 0)); }
     for (long i = tok + n + at; i < a.max_tokens; i += STEP) a.slots[i] = -1;
   }
 }
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(RPB == 1 ? 256 : 512) void page_tables_extend_kerne
 extern "C" int unimp_page_tables_extend(int32_t* tables, int rows, int width, const int32_t* mapped, const int32_t* cached, const int32_t* fresh, const int32_t* cover,
                                         const int32_t* free_pages, int n_free, const int32_t* cursor, int group, const int32_t* shared_len, int32_t* mapped_out,
                                         int32_t* cursor_out, int64_t* slots, int64_t max_tokens, int32_t* cu, void* stream) {
-  if (!tables || !mapped || !cached || !fresh || !free_pages || !cursor || !mapped_out || !cursor_out || !cu || (max_tokens > 0 && !slots))
+  if (!tables || !mapped || !cached || !fresh || (!free_pages && n_free > 0) || !cursor || !mapped_out || !cursor_out || !cu || (max_tokens > 0 && !slots))
     return unimp_set_error(UNIMP_ERR_ARG, "page_tables_extend: null pointer");
   if (rows <= 0 || rows > 65536 || width <= 0 || n_free < 0 || max_tokens < 0 || group < 1 || (rows % group))      // every workgroup sums over the rows before it
     return unimp_set_error(UNIMP_ERR_SHAPE, "page_tables_extend: rows a positive multiple of group, at most 65536; width positive");
@@ -522,10 +523,10 @@ __global__ __launch_bounds__(256) void kv4_reorder_beams_kernel(uint8_t* __restr
 
 extern "C" int unimp_kv4_reorder_beams(void* pages, int64_t layer_stride, int layers, int64_t n_pages, int heads, int hd, int32_t* tables, int width, int group,
                                        int n_groups, const int64_t* src_local, const int64_t* pos, void* stream) {
-  if (!pages || !tables || !src_local || !pos) return unimp_set_error(UNIMP_ERR_ARG, "kv4_reorder_beams: null pointer");
   const int pb = unimp_kv4_page_bytes(hd);
   if (pb < 0) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4: head dim 64, 80 or 128");
-  if (layers <= 0 || n_groups <= 0 || group <= 1 || width <= 0) return UNIMP_OK;
+  if (layers <= 0 || n_groups <= 0 || group <= 1 || width <= 0) return UNIMP_OK;          // empty tensors have no pointers
+  if ((!pages && n_pages > 0 && heads > 0) || !tables || !src_local || !pos) return unimp_set_error(UNIMP_ERR_ARG, "kv4_reorder_beams: null pointer");
   if (group > 16 || layers > 65535 || n_groups > 65535) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_reorder_beams: at most 16 beams, 65535 layers and groups");
   if (((uintptr_t)pages | layer_stride) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_reorder_beams: 16-byte aligned pages and layer stride");
   const long stride = (long)heads * pb;

@@ -1115,14 +1115,14 @@ def _kv4_fn(name):
 
 
 def _kv4_rows(t):
-    """a [tokens, heads, hd] bf16 view whose 8-element pieces are 16-byte aligned (copied only if it is not one)"""
+    """a [tokens, heads, hd] bf16 view whose 8-element pieces are 16-byte aligned (copied only if it is not one; contiguous() would hand a misaligned one back)"""
     st = t.stride()
-    return t if st[2] == 1 and not (st[0] & 7 or st[1] & 7 or t.data_ptr() & 15) else t.contiguous()
+    return t if st[2] == 1 and not (st[0] & 7 or st[1] & 7 or t.data_ptr() & 15) else t.clone(memory_format=torch.contiguous_format)
 
 
 def kv4_write(k, v, pages, slots):
     """quantise k and v [tokens, heads, hd] (bf16 views, e.g. a prefill's rotated keys) into the slots [tokens] (int64; slot s = token s % 32 of page s // 32; a slot
-    outside the pool: the token is not written) of one layer's pages [n_pages, heads, kv4_page_bytes(hd)]."""
+    outside the pool: the token is not written; the others all different) of one layer's pages [n_pages, heads, kv4_page_bytes(hd)]."""
     shape, pool = k.shape, pages.shape
     if not (len(shape) == 3 and shape == v.shape and k.dtype is bf16 and v.dtype is bf16 and len(pool) == 3 and pages.dtype is _u8 and pages.is_contiguous()
             and pool[1] == shape[1] and pool[2] == _KV4_BYTES.get(shape[2]) and slots.dtype is _i64 and slots.shape == shape[:1] and slots.is_contiguous()):
@@ -1135,7 +1135,7 @@ def kv4_write(k, v, pages, slots):
 
 def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows, pages, slots):
     """decode step on the 4-bit cache: rotate q and k of every row (row r with ITS table row cos_rows / sin_rows [rows, rot // 2]; rot = 0: none), quantise the
-    rotated k and v into slot slots[r] of one layer's pages, return the rotated q [rows, heads, hd].  Operand layout of decode_rope_append; qkv2d is left unrotated."""
+    rotated k and v into slot slots[r] (different ones) of one layer's pages, return the rotated q [rows, heads, hd].  Operand layout of decode_rope_append; qkv2d is left unrotated."""
     rows, width = qkv2d.shape
     stride, unit = qkv2d.stride()
     q_off, k_off, v_off = offs
@@ -1143,7 +1143,7 @@ def kv4_rope_append(qkv2d, heads, head_stride, hd, offs, rot, cos_rows, sin_rows
     if not (qkv2d.dtype is bf16 and unit == 1 and len(pool) == 3 and pages.dtype is _u8 and pages.is_contiguous() and pool[1] == heads
             and pool[2] == _KV4_BYTES.get(hd) and min(q_off, k_off, v_off, head_stride) >= 0 and max(q_off, k_off, v_off) + (heads - 1) * head_stride + hd <= width
             and slots.dtype is _i64 and slots.shape == (rows,) and slots.is_contiguous()
-            and (rot == 0 or (0 < rot <= hd and not rot & 1 and cos_rows.dtype is _f32 and sin_rows.dtype is _f32 and cos_rows.shape == (rows, rot // 2) == sin_rows.shape
+            and (rot == 0 or (0 < rot <= hd and not rot & 1 and cos_rows is not None and sin_rows is not None and cos_rows.dtype is _f32 and sin_rows.dtype is _f32 and cos_rows.shape == (rows, rot // 2) == sin_rows.shape
                               and cos_rows.is_contiguous() and sin_rows.is_contiguous()))):
         _kv4_refuse("kv4_rope_append", "qkv bf16 rows with q, k, v of every head inside; pages contiguous uint8 [n_pages, heads, kv4_page_bytes(hd)]; slots contiguous int64 [rows]; "
                     "rot even, at most hd; cos, sin contiguous fp32 [rows, rot // 2]", qkv=qkv2d, heads=heads, head_stride=head_stride, hd=hd, offs=offs, rot=rot, cos=cos_rows,
@@ -1256,7 +1256,7 @@ def kv4_attn_decode(q, pages, tables, lens, scale, alibi=None, group=1, shared_l
     rows, heads, hd = shape
     qr, qh, unit = q.stride()
     if unit != 1 or qr & 7 or qh & 7 or q.data_ptr() & 15:                            # no 16-byte loads from this view
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)
         qr, qh, _ = q.stride()
     if out is None:
         out = q.new_empty(shape)
