@@ -44,17 +44,24 @@ def check(got, want, bound, name=""):
 
 # ------------------------------------------------------------------------------------------------- write, read
 @pytest.mark.parametrize("hd", [64, 80, 128])
-@pytest.mark.parametrize("tokens,heads,order", [(1, 1, "run"), (31, 3, "run"), (32, 2, "run"), (33, 2, "offset"), (100, 4, "offset"), (257, 2, "gaps"), (97, 3, "random")])
+@pytest.mark.parametrize("tokens,heads,order", [(1, 1, "run"), (31, 3, "run"), (32, 2, "run"), (33, 2, "offset"), (100, 4, "offset"), (257, 2, "gaps"), (97, 3, "random"), (400, 5, "pieces")])
 def test_write_read(ops, hd, tokens, heads, order):
-    """runs that start anywhere in a page, with padding between requests, and slots in random order; nothing but the named slots changes"""
-    n_pages = (tokens + 40) // 32 + 3
+    """runs of any length that start anywhere in a page, with padding between requests, and slots in random order; nothing but the named slots changes"""
+    n_pages = (tokens + 40) // 32 + 3 if order != "pieces" else tokens
     g = torch.Generator().manual_seed(tokens)
     page = torch.randperm(n_pages, generator=g)
-    first = {"run": 0, "offset": 13, "gaps": 5, "random": 0}[order]
+    first = {"run": 0, "offset": 13, "gaps": 5, "random": 0, "pieces": 0}[order]
     t = torch.arange(first, first + tokens)
     slots = page[t // 32] * 32 + t % 32
     if order == "random":
         slots = torch.randperm(n_pages * 32, generator=g)[:tokens]
+    if order == "pieces":                                           # runs of 1 ... 16 tokens anywhere in their pages: whole, or in two parts the second of which comes first
+        parts = []
+        for pg in page.tolist():
+            a, n = (int(x) for x in torch.randint(1, 17, (2,), generator=g))
+            r = pg * 32 + a - 1 + torch.arange(n)
+            parts.append(r if pg % 3 else torch.cat([r[n // 2:], r[:n // 2]]))
+        slots = torch.cat(parts)[:tokens].contiguous()
     if order == "gaps":
         slots[torch.rand(tokens, generator=g) < 0.2] = -1
         slots[7] = n_pages * 32

@@ -21,21 +21,43 @@ extern "C" int unimp_kv4_page_bytes(int hd) { return hd == 64 || hd == 80 || hd 
 // ------------------------------------------------------------------------------------------- runs of slots
 // A RUN is a maximal stretch of consecutive rows whose slots are consecutive inside one page; a workgroup (chunk of 32 rows, some heads) owns the runs that START
 // in its chunk (a run has at most 32 rows: it looks 31 rows ahead), so every row is moved once and every page is touched by one wave per run, whatever the
-// alignment of the rows to the pages.  sl[1 + i] = slot of row i0 + i, -1: none.
-__device__ __forceinline__ void kv4_load_slots(int64_t (&sl)[65], const int64_t* __restrict__ slots, long i0, long tokens, long n_pages) {
-  if (threadIdx.x < 65) {
-    const long i = i0 - 1 + (int)threadIdx.x;
+// alignment of the rows to the pages.  A run shorter than KV4_SHORT rows costs its latencies whatever its length: the rows of such runs are moved one by one, all of a chunk's
+// at once.  Measured, 16 384 tokens x 32 heads x 80 dims in runs of 8 | 11 | 12 | 15, write: as rows 91 | 90 | 88 | 88 us, as runs 127 | 103 | 97 |
+// 86; 33 requests of 1 or 2 tokens x 32 heads x 128, write and read back: 116 -> 16 us.  sl[KV4_BACK + i] = slot of row i0 + i, -1: none.
+#define KV4_SHORT 12
+#define KV4_BACK 12
+#define KV4_SLOTS (KV4_BACK + 64)
+__device__ __forceinline__ void kv4_load_slots(int64_t (&sl)[KV4_SLOTS], const int64_t* __restrict__ slots, long i0, long tokens, long n_pages) {
+  if (threadIdx.x < KV4_SLOTS) {
+    const long i = i0 - KV4_BACK + (int)threadIdx.x;
     const int64_t s = i >= 0 && i < tokens ? slots[i] : -1;
     sl[threadIdx.x] = s >= 0 && s < n_pages * KV4_PAGE ? s : -1;
   }
   __syncthreads();
 }
-// rows of the run that starts at row a (0: none starts there)
-__device__ __forceinline__ int kv4_run(const int64_t (&sl)[65], int a) {
-  const int64_t s0 = sl[a + 1];
-  if (s0 < 0 || !(sl[a] < 0 || sl[a] + 1 != s0 || (s0 & 31) == 0)) return 0;
+// rows of a workgroup's chunk: 32; 8 where that leaves the chip empty (64 tokens x 32 heads x 128 in runs of 1: 19.5 -> 8.9 us, read 15.3 -> 8.0)
+static int kv4_chunk_rows(int64_t tokens, int64_t blocks) { return (tokens + 31) / 32 * blocks <= 256 ? 8 : 32; }      // blocks: of heads, times layers
+// a chunk's rows as bits: `few` belong to runs of less than KV4_SHORT rows, a longer run begins at `starts`, `none` have no slot; `links` go on where the row before ends
+struct Kv4Rows { uint32_t few, starts, none, links; };
+__device__ __forceinline__ Kv4Rows kv4_rows(const int64_t (&sl)[KV4_SLOTS], int rows) {
+  const int lane = lane_id();
+  const int64_t s = sl[lane];
+  const uint64_t link = __ballot(lane > 0 && s >= 0 && (s & 31) && sl[max(lane - 1, 0)] + 1 == s);      // bit l: row i0 - KV4_BACK + l
+  const int at = KV4_BACK + (lane & 31);
+  const int back = __builtin_clzll(~(link << (63 - at))), on = __builtin_ctzll(~(link >> (at + 1)));   // link's lowest bit is 0, and its shifts bring zeros in
+  const bool has = lane < rows && sl[at] >= 0, few = back + on + 1 < KV4_SHORT;
+  Kv4Rows r;
+  r.few = (uint32_t)__ballot(has && few);
+  r.starts = (uint32_t)__ballot(has && !few && !back);
+  r.none = (uint32_t)__ballot(lane < rows && !has);
+  r.links = (uint32_t)(link >> KV4_BACK);
+  return r;
+}
+// rows of the run that starts at row a
+__device__ __forceinline__ int kv4_run(const int64_t (&sl)[KV4_SLOTS], int a) {
+  const int64_t s0 = sl[KV4_BACK + a];
   const int lane = lane_id(), t0 = (int)(s0 & 31);
-  const bool on = lane < 32 && a + lane < 64 && t0 + lane < 32 && sl[min(a + 1 + lane, 64)] == s0 + lane;      // lane 0: itself
+  const bool on = lane < 32 && t0 + lane < 32 && sl[KV4_BACK + a + (lane & 31)] == s0 + lane;      // lane 0: itself
   return __builtin_ctzll(~__ballot(on));
 }
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
@@ -73,25 +95,107 @@ __device__ __forceinline__ void wave_lds_fence() {                   // LDS of t
 #define KV4_HEADS 4                                                  // heads of a workgroup; the head blocks of a chunk are neighbours in the grid (whole rows in flight)
 template <int D>
 __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long k_ts, long k_hs, long v_ts, long v_hs,
-                                                           uint8_t* __restrict__ pages, long n_pages, int heads, int head_blocks, const int64_t* __restrict__ slots, long tokens) {
+                                                           uint8_t* __restrict__ pages, long n_pages, int heads, int head_blocks, int chunk_rows, const int64_t* __restrict__ slots, long tokens) {
   using P = Kv4<D>;
   constexpr int X = D / 8, TP = 16 / P::NB, PASSES = (32 + TP - 1) / TP;      // 8-dim pieces of a row; tokens of a pass (four lanes to a block)
-  __shared__ int64_t sl[65];
+  __shared__ int64_t sl[KV4_SLOTS];
   __shared__ __attribute__((aligned(16))) uint8_t image[4][P::BYTES];
   __shared__ uint32_t turn[4][32 * X];
+  __shared__ int piece[4][32];
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane & 3;
   const int tl = (lane >> 2) / P::NB, b = (lane >> 2) - tl * P::NB, d = 32 * b + 8 * quad;      // this lane's token of a pass, block and dims
   const bool on = tl < TP && d < D;
   const long lane_k = tl * k_ts + d, lane_v = tl * v_ts + d;
-  const long chunk = blockIdx.x / head_blocks, i0 = chunk * 32;
+  const long chunk = blockIdx.x / head_blocks, i0 = chunk * chunk_rows;
   const int h0 = (blockIdx.x - (unsigned)chunk * head_blocks) * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
   kv4_load_slots(sl, slots, i0, tokens, n_pages);
   uint8_t* im = image[w];
   uint32_t* tv = turn[w];
-  for (int a = 0; a < 32;) {
-    const int n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
-    if (!n) { ++a; continue; }                                       // no slot, or the tail of the previous chunk's last run
-    const int64_t s0 = uniform64(sl[a + 1]);
+  // four lanes' 8 elements each of one block -> this lane's codes and the scale byte
+  auto quantise = [](const bf16x8& u, int& sb) {
+    float f[8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { f[j] = bf2f(u[j]); m = max(m, __float_as_uint(f[j]) & 0x7fffffffu); }
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));       // lane ^ 1
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));       // lane ^ 2
+    sb = kv4_scale_byte((int)(m >> 23));
+    const float scale = __uint_as_float((uint32_t)(sb == 255 ? 127 : sb) << 23);
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[0], f[1], scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[2], f[3], scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[4], f[5], scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[6], f[7], scale, 3);
+    return sb == 255 ? 0u : r;
+  };
+  const Kv4Rows rows = kv4_rows(sl, chunk_rows);
+  if (const uint32_t few = rows.few, links = rows.links; few) {
+    constexpr bool PAIR = P::NI % 2 == 0;
+    constexpr int U = PAIR ? D / 2 : D;
+    const uint32_t quarter = (uint32_t)__ballot(lane < 32 && !(sl[KV4_BACK + (lane & 31)] & 3)) | 1u;      // row 0 and tokens 0, 4, ... of a page start a piece in any case
+    const int n_pieces = __builtin_popcount(few & ~(links & ~quarter));
+    for (int head = h0 + w; head < h1; head += 4) {
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const long ts = kind ? v_ts : k_ts;
+        const bf16* mine = (kind ? v + head * v_hs + lane_v : k + head * k_hs + lane_k) + i0 * ts;
+        bf16x8 u[PASSES];
+#pragma unroll
+        for (int ps = 0; ps < PASSES; ++ps) {
+          const int i = ps * TP + tl;
+          u[ps] = bf16x8{};
+          if (on && i < 32 && (few >> i & 1)) u[ps] = *(const bf16x8*)(mine + ps * TP * ts);
+        }
+#pragma unroll
+        for (int ps = 0; ps < PASSES; ++ps) {
+          if (!(few >> (ps * TP) & ((1u << TP) - 1))) continue;      // uniform
+          const int i = ps * TP + tl;
+          int sb;
+          const uint32_t r = quantise(u[ps], sb);
+          if (on && i < 32 && (few >> i & 1)) {
+            const int64_t slot = sl[KV4_BACK + i];
+            const int t = (int)(slot & 31);
+            uint8_t* page = pages + ((slot >> 5) * heads + head) * (long)P::BYTES;
+            if (!quad) page[kind ? P::vs_byte(t, b) : P::ks_byte(t, b)] = (uint8_t)sb;
+            if (!kind) *(uint32_t*)(page + P::k_byte(t, b) + 4 * quad) = r;
+            else tv[i * X + (d >> 3)] = r;
+          }
+        }
+      }
+      // V: up to four consecutive tokens share their dwords (a piece); consecutive lanes take consecutive dwords, two at a time where a token's dwords pair up
+      if (lane < 32) {
+        const uint32_t starts = few & ~(links & ~quarter);
+        if (starts >> lane & 1) piece[w][__builtin_popcount(starts & ((1u << lane) - 1))] = lane | (__builtin_ctz(~((links & ~quarter & few) >> 1 >> lane)) + 1) << 8;
+      }
+      wave_lds_fence();
+      const int units = n_pieces * U;
+      for (int x = lane; x < units; x += 64) {
+        const int pc = piece[w][x / U], first = pc & 255, len = pc >> 8, un = x % U;
+        const int64_t slot = sl[KV4_BACK + first];
+        const int t = (int)(slot & 31), sh = 4 * kv4_nibble(t);
+        uint8_t* page = pages + ((slot >> 5) * heads + head) * (long)P::BYTES;
+        const int dim = PAIR ? 32 * (un % (P::NI / 2)) + un / (P::NI / 2) : 16 * (un % P::NI) + un / P::NI;
+        uint32_t lo = 0, hi = 0;
+        for (int e = 0; e < len; ++e) {
+          const uint32_t* row = tv + (first + e) * X;
+          lo |= (row[dim >> 3] >> (4 * (dim & 7)) & 15u) << (4 * e);
+          if (PAIR) hi |= (row[(dim >> 3) + 2] >> (4 * (dim & 7)) & 15u) << (4 * e);
+        }
+        const uint32_t mask = (0xffffu >> (16 - 4 * len)) << sh;
+        if constexpr (PAIR) {
+          unsigned long long* o = (unsigned long long*)(page + P::v_dword(t, dim));
+          atomicAnd(o, ~(mask * 0x100000001ull)); atomicOr(o, (unsigned long long)(lo << sh) | (unsigned long long)(hi << sh) << 32);
+        } else {
+          uint32_t* o = (uint32_t*)(page + P::v_dword(t, dim));
+          atomicAnd(o, ~mask); atomicOr(o, lo << sh);
+        }
+      }
+      wave_lds_fence();
+    }
+  }
+  for (uint32_t todo = rows.starts; todo; todo &= todo - 1) {
+    const int a = __builtin_ctz(todo), n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
+    const int64_t s0 = uniform64(sl[KV4_BACK + a]);
     const int t0 = (int)(s0 & 31);
     const long row0 = i0 + a - t0;                                   // the row that page token 0 has or would have
     for (int head = h0 + w; head < h1; head += 4) {
@@ -111,20 +215,8 @@ __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restric
 #pragma unroll
         for (int ps = 0; ps < PASSES; ++ps) {
           const int t = ps * TP + tl;
-          float f[8];
-          uint32_t m = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) { f[j] = bf2f(u[ps][j]); m = max(m, __float_as_uint(f[j]) & 0x7fffffffu); }
-          m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));       // lane ^ 1
-          m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));       // lane ^ 2
-          const int sb = kv4_scale_byte((int)(m >> 23));
-          const float scale = __uint_as_float((uint32_t)(sb == 255 ? 127 : sb) << 23);
-          uint32_t r = 0;
-          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[0], f[1], scale, 0);
-          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[2], f[3], scale, 1);
-          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[4], f[5], scale, 2);
-          r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, f[6], f[7], scale, 3);
-          if (sb == 255) r = 0;
+          int sb;
+          const uint32_t r = quantise(u[ps], sb);
           if (on && t < 32) {
             if (!kind) *(uint32_t*)(im + P::k_byte(t, b) + 4 * quad) = r;
             else tv[t * X + (d >> 3)] = r;
@@ -168,7 +260,6 @@ __global__ __launch_bounds__(256, 4) void kv4_write_kernel(const bf16* __restric
       }
       wave_lds_fence();
     }
-    a += n;
   }
 }
 
@@ -177,12 +268,13 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
   if (tokens <= 0 || heads <= 0 || n_pages <= 0) return UNIMP_OK;
   if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
+  const int cr = kv4_chunk_rows(tokens, hb);
   if (heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^31 token heads");
   if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
     return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_write: strides multiples of 8 elements, 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
-    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + 31) / 32 * hb)), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
-                       (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, (int)hb, slots, (long)tokens);
+    hipLaunchKernelGGL((kv4_write_kernel<decltype(d)::value>), dim3((unsigned)((tokens + cr - 1) / cr * hb)), dim3(256), 0, (hipStream_t)stream, (const bf16*)k,
+                       (const bf16*)v, (long)k_ts, (long)k_hs, (long)v_ts, (long)v_hs, (uint8_t*)pages, (long)n_pages, heads, (int)hb, cr, slots, (long)tokens);
     return unimp_check_launch("kv4_write");
   });
 }
@@ -282,14 +374,14 @@ extern "C" int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_
 // A wave per (run, head): every page is read once, whatever rows name its tokens.  K: a lane converts 8 dims of a token; V: a lane takes 8 tokens x 8 dims, turns the
 // nibbles round in registers and stores 16 bytes of each token.  Bound by the bf16 rows that leave.
 template <int D>
-__global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, int head_blocks,
+__global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restrict__ pages, long layer_stride, long n_pages, int heads, int head_blocks, int chunk_rows,
                                                           const int64_t* __restrict__ slots, long tokens, bf16* __restrict__ k, bf16* __restrict__ v) {
   using P = Kv4<D>;
   constexpr int X = D / 8, TP = 64 / X, PASSES = (32 + TP - 1) / TP;          // 8-dim pieces of a row; tokens of a pass
-  __shared__ int64_t sl[65];
+  __shared__ int64_t sl[KV4_SLOTS];
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tl = lane / X, d = (lane - tl * X) * 8, b = d >> 5;               // K: this lane's token of a pass and dims; V: tl = group g of 8 tokens
-  const long chunk = blockIdx.x / head_blocks, i0 = chunk * 32;
+  const long chunk = blockIdx.x / head_blocks, i0 = chunk * chunk_rows;
   const int h0 = (blockIdx.x - (unsigned)chunk * head_blocks) * KV4_HEADS, h1 = min(h0 + KV4_HEADS, heads);
   kv4_load_slots(sl, slots, i0, tokens, n_pages);
   const long lo = (long)blockIdx.y * tokens;
@@ -302,19 +394,38 @@ __global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restr
     if (byte == 255u) { const uint32_t nn = 0x7fc07fc0u; u.h[0] = u.h[1] = u.h[2] = u.h[3] = __builtin_bit_cast(bf16x2, nn); }
     return u.v;
   };
-  for (int a = 0; a < 32 && i0 + a < tokens;) {
-    const int64_t s0 = uniform64(sl[a + 1]);
-    if (s0 < 0) {                                                    // no slots: rows of zeros, up to the next slot
-      const int end = (int)min(32l, tokens - i0);
-      const int z = __builtin_ctzll(~__ballot(lane < 32 && a + lane < end && sl[min(a + 1 + lane, 64)] < 0)), per = (h1 - h0) * X;
-      for (int x = threadIdx.x; x < z * per; x += 256) {
-        const long o = (lo + i0 + a + x / per) * row + h0 * D + 8 * (x % per);
-        *(bf16x8*)(k + o) = bf16x8{}; *(bf16x8*)(v + o) = bf16x8{};
-      }
-      a += z; continue;
+  const Kv4Rows rows = kv4_rows(sl, chunk_rows);
+  if (rows.none) {                                                   // no slots: rows of zeros
+    const int per = (h1 - h0) * X, end = (int)min((long)chunk_rows, tokens - i0);
+    for (int x = threadIdx.x; x < end * per; x += 256) if (rows.none >> (x / per) & 1) {
+      const long o = (lo + i0 + x / per) * row + h0 * D + 8 * (x % per);
+      *(bf16x8*)(k + o) = bf16x8{}; *(bf16x8*)(v + o) = bf16x8{};
     }
-    const int n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
-    if (!n) { ++a; continue; }                                       // the previous chunk's
+  }
+  if (const uint32_t few = rows.few) {
+    for (int head = h0 + w; head < h1; head += 4) {
+#pragma unroll 2
+      for (int ps = 0; ps < PASSES; ++ps) {
+        if (!(few >> (ps * TP) & ((1u << TP) - 1))) continue;        // uniform
+        const int i = ps * TP + tl;
+        if (tl < TP && i < 32 && (few >> i & 1)) {
+          const int64_t slot = sl[KV4_BACK + i];
+          const int t = (int)(slot & 31), sh = 4 * kv4_nibble(t);
+          const uint8_t* page = pages + (long)blockIdx.y * layer_stride + ((slot >> 5) * heads + head) * (long)P::BYTES;
+          const long o = (lo + i0 + i) * row + head * D + d;
+          const uint32_t c = *(const uint32_t*)(page + P::k_byte(t, b) + ((d & 31) >> 1)), ks = page[P::ks_byte(t, b)], vs = page[P::vs_byte(t, b)];
+          uint32_t y = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y |= (*(const uint32_t*)(page + P::v_dword(t, d + j)) >> sh & 15u) << (4 * j);
+          *(bf16x8*)(k + o) = values(c, ks);
+          *(bf16x8*)(v + o) = values(y, vs);
+        }
+      }
+    }
+  }
+  for (uint32_t todo = rows.starts; todo; todo &= todo - 1) {
+    const int a = __builtin_ctz(todo), n = __builtin_amdgcn_readfirstlane(kv4_run(sl, a));
+    const int64_t s0 = uniform64(sl[KV4_BACK + a]);
     const int t0 = (int)(s0 & 31);
     for (int head = h0 + w; head < h1; head += 4) {
       const uint8_t* page = pages + (long)blockIdx.y * layer_stride + ((s0 >> 5) * heads + head) * (long)P::BYTES;
@@ -346,7 +457,6 @@ __global__ __launch_bounds__(256, 4) void kv4_read_kernel(const uint8_t* __restr
         }
       }
     }
-    a += n;
   }
 }
 
@@ -355,13 +465,14 @@ extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layer
   if (tokens <= 0 || heads <= 0 || layers <= 0) return UNIMP_OK;
   if ((!pages && n_pages > 0) || !slots || !k || !v) return unimp_set_error(UNIMP_ERR_ARG, "kv4_read: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
+  const int cr = kv4_chunk_rows(tokens, hb * layers);
   if (layers > 65535 || heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23)
     return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^31 token heads");
   if (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_read: 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens + 31) / 32 * hb), layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
-                       (long)layer_stride, (long)n_pages, heads, (int)hb, slots, (long)tokens, (bf16*)k, (bf16*)v);
+    hipLaunchKernelGGL((kv4_read_kernel<D>), dim3((unsigned)((tokens + cr - 1) / cr * hb), layers), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)pages,
+                       (long)layer_stride, (long)n_pages, heads, (int)hb, cr, slots, (long)tokens, (bf16*)k, (bf16*)v);
     return unimp_check_launch("kv4_read");
   });
 }
