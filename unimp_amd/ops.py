@@ -1202,7 +1202,7 @@ def page_tables_extend(tables, mapped, cached, new, free_pages, cursor, max_toke
     _kv4_launch("page_tables_extend", (tables, mapped, cached, new, free_pages, cursor, cover, shared_len),
                 (tables.data_ptr(), rows, width, mapped.data_ptr(), cached.data_ptr(), new.data_ptr(), None if cover is None else cover.data_ptr(), free_pages.data_ptr(),
                  free_pages.shape[0], cursor.data_ptr(), group, None if shared_len is None else shared_len.data_ptr(), p, p + 4 * rows, slots.data_ptr(), max_tokens, p + 4 * rows + 4))
-    mapped_out, cursor_out, cu = ints.split((rows, 1, rows + 1))
+    mapped_out, cursor_out, cu = torch.split_with_sizes(ints, (rows, 1, rows + 1))
     return mapped_out, cursor_out, slots, cu
 
 
