@@ -502,46 +502,55 @@ __device__ __forceinline__ PageRow page_row(const PageArgs& a, int r, int& alias
   }
   return PageRow{need, max(map, alias)};
 }
+// sum over a wave's lanes: inside the rows of 16 by lane moves of the vector pipe, the four rows as scalars
+__device__ __forceinline__ long wave_total(long x) {
+  auto moved = [&](auto C) {
+    constexpr int c = decltype(C)::value;
+    return (long)(((uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), c, 0xf, 0xf, true) << 32) | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, c, 0xf, 0xf, true));
+  };
+  x += moved(std::integral_constant<int, 0xB1>()); x += moved(std::integral_constant<int, 0x4E>());      // lane ^ 1, ^ 2
+  x += moved(std::integral_constant<int, 0x141>()); x += moved(std::integral_constant<int, 0x140>());    // mirrored inside 8 and inside 16 lanes
+  long s = 0;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16) s += (long)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, i));
+  return s;
+}
 // RPB = 1: a workgroup per row; 8: a wave per row (the sum over the rows before is made once for eight)
 template <int RPB>
 __global__ __launch_bounds__(RPB == 1 ? 256 : 512) void page_tables_extend_kernel(PageArgs a) {
   constexpr int T = RPB == 1 ? 256 : 512, STEP = RPB == 1 ? T : 64;
   __shared__ long red[2][T / 64];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r0 = blockIdx.x * RPB;
+  const int r = RPB == 1 ? r0 : min(r0 + wave, a.rows - 1);
+  const int first = a.group > 1 ? r / a.group * a.group : r;
+  // the row's own numbers and those of rows [r0, r) and [first, r): requested together with the sum over the rows before
+  const int start = a.cursor[0];
+  int alias, map; const PageRow p = page_row(a, r, alias, map);
+  int al0 = 0, map0 = 0, begin0 = 0;
+  if (first != r) begin0 = page_row(a, first, al0, map0).begin;
+  long in_block = 0, in_block_tok = 0, in_group = 0;
+  for (int i = min(r0, first) + lane; i < r; i += 64) {
+    int al, m; const PageRow q = page_row(a, i, al, m);
+    const int own = max(q.need - q.begin, 0);
+    if (i >= r0) { in_block += own; in_block_tok += max(a.fresh[i], 0); }
+    if (i >= first) in_group += own;
+  }
   long before = 0, tok = 0;                                          // pages taken and tokens packed by the rows [0, r0)
   if (!a.shared) {                                                   // no groups: the loads of eight rows at once
 #pragma unroll 8
     for (int i = tid; i < r0; i += T) { int m; const int need = page_need(a, i, m); before += max(need - m, 0); tok += max(a.fresh[i], 0); }
   } else {
-    for (int i = tid; i < r0; i += T) { int al, m; const PageRow p = page_row(a, i, al, m); before += max(p.need - p.begin, 0); tok += max(a.fresh[i], 0); }
+    for (int i = tid; i < r0; i += T) { int al, m; const PageRow q = page_row(a, i, al, m); before += max(q.need - q.begin, 0); tok += max(a.fresh[i], 0); }
   }
-  auto wave_total = [](long x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
-  };
   before = wave_total(before); tok = wave_total(tok);
   if (!lane) { red[0][wave] = before; red[1][wave] = tok; }
+  if (r > min(r0, first)) { in_block = wave_total(in_block); in_block_tok = wave_total(in_block_tok); in_group = wave_total(in_group); }
   __syncthreads();
-  const int r = RPB == 1 ? r0 : r0 + wave;
-  if (r >= a.rows) return;
-  before = a.cursor[0]; tok = 0;
+  if (RPB > 1 && r0 + wave >= a.rows) return;
+  before = start + in_block; tok = in_block_tok;
 #pragma unroll
   for (int i = 0; i < T / 64; ++i) { before += red[0][i]; tok += red[1][i]; }
-  const int first = a.group > 1 ? r / a.group * a.group : r;
-  long in_block = 0, in_block_tok = 0, in_group = 0;                 // rows [r0, r), rows [first, r)
-  for (int i = min(r0, first) + lane; i < r; i += 64) {
-    int al, m; const PageRow p = page_row(a, i, al, m);
-    const int own = max(p.need - p.begin, 0);
-    if (i >= r0) { in_block += own; in_block_tok += max(a.fresh[i], 0); }
-    if (i >= first) in_group += own;
-  }
-  if (r > min(r0, first)) { in_block = wave_total(in_block); in_block_tok = wave_total(in_block_tok); in_group = wave_total(in_group); }
-  before += in_block; tok += in_block_tok;
   const long before_first = before - in_group;
-  int alias, map; const PageRow p = page_row(a, r, alias, map);
-  int al0 = 0, map0 = 0, begin0 = 0;
-  if (first != r) begin0 = page_row(a, first, al0, map0).begin;
   const int32_t* row0 = a.tables + (long)first * a.width;
   int32_t* row = a.tables + (long)r * a.width;
   auto from_free = [&](long i) { return i >= 0 && i < a.n_free ? a.free_pages[i] : -1; };
