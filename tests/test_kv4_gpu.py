@@ -237,7 +237,8 @@ def test_reorder_beams(ops, K, groups, heads, hd, layers):
 @pytest.mark.parametrize("rows,kvh,G,lens,alibi", [
     (1, 1, 1, [1], False), (5, 2, 1, [0, 1, 31, 32, 33], True), (3, 3, 2, [64, 7, 200], False), (2, 1, 16, [129, 300], True), (4, 2, 3, [96, 0, 1, 511], True),
     (2, 4, 8, [1500, 40], False), (1, 2, 1, [4500], True), (70, 16, 1, [5, 130, 64, 0, 513, 31, 200], False), (40, 32, 2, [77, 1, 90, 0], True),
-    (9, 2, 4, [3000, 0, 1777, 2111], True), (3, 2, 6, [700, 33, 0], True), (1, 1, 5, [2500], False), (2, 1, 9, [95, 400], True)])
+    (9, 2, 4, [3000, 0, 1777, 2111], True), (3, 2, 6, [700, 33, 0], True), (1, 1, 5, [2500], False), (2, 1, 9, [95, 400], True),
+    (9, 32, 1, [1400, 5, 300, 0, 64, 700, 31, 1, 1290], True)])
 def test_attention(ops, hd, rows, kvh, G, lens, alibi):
     lens = (lens * rows)[:rows]
     W = (max(lens) + 31) // 32 + 1

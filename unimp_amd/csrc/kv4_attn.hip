@@ -410,7 +410,10 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
   p.gmode = mode(p.group * G);
-  p.nw = p.mode >= 2 || p.group > 1 ? 4 : units <= 256 && d->width <= (units > 64 ? 48 : 32) ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
+  // waves of a workgroup: eight where a row is one chunk and workgroups are few -- up to 256 pairs, and up to 512 of head dim 64 and 80, whose registers let two such workgroups share a
+  // CU (512 pairs x 80 dims of up to 2 048 tokens: four waves 17.0 us, eight 15.6, all of 2 048 19.7 | 19.2; of 128 dims 17.2 | 19.4); one where rows are short and many
+  const bool few = units <= 256 ? d->width <= (units > 64 ? 48 : 32) : units <= 512 && d->hd < 128 && d->width > 40 && d->width <= 64;
+  p.nw = p.mode >= 2 || p.group > 1 ? 4 : few ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
   // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 66.7 us, 48 61.6, 64 67.4, 96 61.8).
   // Fewer: one chunk where a wave has few pages then (no merge: 8 query heads to a key head, 20 pages: 9.5 -> 8.4 us; 128 pairs x 47 pages, eight waves: 11.8 -> 10.2), else as many
   // as make 512 workgroups of at least 16 pages (128 pairs x 157 pages: 4 chunks 17.2 us, 5 18.8, 8 20.6; 256 x 50: 2 chunks 13.0, 3 15.5; 32 x 63: 4 chunks 9.1, 2 11.4)
