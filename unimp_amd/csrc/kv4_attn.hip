@@ -74,9 +74,9 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
     const bf16* qp = a.q + (long)my_row * a.q_rs + (long)my_head * a.q_hs;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool in = qi < nq && 64 * h + 16 * g < D;
-      qu[2 * h] = in ? *(const bf16x8*)(qp + 64 * h + 16 * g) : bf16x8{};
-      qu[2 * h + 1] = in ? *(const bf16x8*)(qp + 64 * h + 16 * g + 8) : bf16x8{};
+      const bf16* part = qp + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0);        // behind the head: loaded from its start, zeroed below (a masked load would end the others' flight)
+      qu[2 * h] = *(const bf16x8*)part;
+      qu[2 * h + 1] = *(const bf16x8*)(part + 8);
     }
   }
   const int shared = a.group > 1 ? min(max(a.shared[row / a.group], 0) / KV4_PAGE, a.width) : 0;
@@ -104,23 +104,18 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   const int n = c1 > c0 + w ? (c1 - c0 - w + NW - 1) / NW : 0;                    // pages of this wave
   if (ids >= a.n_pages) ids = -1;
 
-  const uint32_t k_at = P::BLK_LAST < 32 && g == P::NB - 1 ? 512 * g + 8 * col : 512 * g + 16 * col, ks_at = P::KS + 32 * g + 2 * col;
+  // lanes of blocks behind the head, and the upper half of a 16-wide last block, hold whatever is there (the next bytes of the page): the query is zero in those dims
+  const int gk = min(g, P::NB - 1), half_block = P::BLK_LAST < 32 && gk == P::NB - 1;
+  const uint32_t k_at = 512 * gk + (half_block ? 8 : 16) * col, k_step = half_block ? 128 : 256, ks_at = P::KS + 32 * gk + 2 * col;
   const uint32_t v_at = P::VOFF + 4 * (g * D + col * NI), vs_at = P::VS + 8 * P::NB * g + 8 * min(MODE == 0 ? var >> 1 : MODE == 1 ? var : col & 3, P::NB - 1);
   auto page_of = [&](int k) { return a.pages + ((long)max(__builtin_amdgcn_readlane(ids, k), 0) * a.kv_heads + kvh) * P::BYTES; };
   // every lane's loads of page k, unconditional (past the last page: that one again, from the cache), so that the number in flight is known everywhere
   auto load = [&](Kv4Frag<D>& f, int k) {
     const uint8_t* page = page_of(min(k, n - 1));
+    typedef __attribute__((ext_vector_type(4), aligned(8))) uint32_t u32x4h;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (D == 128) f.k[h] = *(const u32x4*)(page + k_at + 256 * h);
-      else {
-        f.k[h] = u32x4{0, 0, 0, 0};
-        if (g < P::NB - (P::BLK_LAST < 32)) f.k[h] = *(const u32x4*)(page + k_at + 256 * h);
-        else if (P::BLK_LAST < 32 && g == P::NB - 1) { const u32x2 t = *(const u32x2*)(page + k_at + 128 * h); f.k[h] = u32x4{t[0], t[1], 0, 0}; }
-      }
-    }
-    f.ks = 0x7f7f;
-    if (D == 128 || g < P::NB) f.ks = *(const uint16_t*)(page + ks_at);
+    for (int h = 0; h < 2; ++h) f.k[h] = *(const u32x4h*)(page + k_at + k_step * h);
+    f.ks = *(const uint16_t*)(page + ks_at);
     if constexpr (D == 80) {
       typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4u;
       f.v0 = *(const u32x4u*)(page + v_at); f.v1[0] = *(const uint32_t*)(page + v_at + 16);
@@ -132,7 +127,12 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   };
 
   Kv4Frag<D> fa, fb;
-  if (n > 0) { load(fa, 0); load(fb, 1); }
+  if (n > 0) {                                                                    // in this order: the loop counts them
+    load(fa, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(fb, 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 
   i32x8 qh, ql;
   int sb;
@@ -142,9 +142,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
     for (int h = 0; h < 2; ++h) {
       float x[16];
       uint32_t mx = 0;
+      const bool in = qi < nq && 64 * h + 16 * g < D;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        x[j] = bf2f(qu[2 * h + (j >> 3)][j & 7]);
+        x[j] = in ? bf2f(qu[2 * h + (j >> 3)][j & 7]) : 0.f;
         mx = max(mx, __float_as_uint(x[j]) & 0x7fffffffu);
       }
       mx = max(mx, __shfl_xor(mx, 16, 64));                                       // the other half of the 32-dim block
@@ -293,8 +294,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   for (int k = 0; k + 1 < n; k += 2) {
     compute(fa, k);
     load(fa, k + 2);
+    __builtin_amdgcn_sched_barrier(0);                                            // requested before the wait for the other page
     compute(fb, k + 1);
     load(fb, k + 3);
+    __builtin_amdgcn_sched_barrier(0);
   }
   if (n & 1) compute(fa, n - 1);
 
