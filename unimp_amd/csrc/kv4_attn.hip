@@ -169,6 +169,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   }
   const float sc = a.scale * 1.4426950408889634f, slope = ALIBI ? a.alibi[my_head] * 1.4426950408889634f : 0.f;
 
+  const uint32_t lo_mask = (MODE == 0 ? var & 1 : var) ? 0xffff0000u : 0u;
   f32x4 acc[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -214,16 +215,27 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][e] *= r;
     }
-    float hi[8], lo[8];
+    float hi[8];
+    [[maybe_unused]] float lo[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float p = __builtin_amdgcn_exp2f(x[j] - mu);
       l += p;
-      hi[j] = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
-      lo[j] = p - hi[j];
+      // pack() drops the lower half: p itself is the high part.  MODE 0 and 3: hi is the part that this lane's column holds
+      if constexpr (MODE == 0 || MODE == 3) hi[j] = p - __uint_as_float(__float_as_uint(p) & lo_mask);
+      else { hi[j] = p; lo[j] = p - __uint_as_float(__float_as_uint(p) & 0xffff0000u); }
     }
     auto pack = [](float a0, float a1) { return __builtin_amdgcn_perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u); };      // upper halves
-    auto vscale = [&](uint32_t d, int j) { return __uint_as_float(((d >> (8 * j)) & 0xffu) << 23); };      // byte 255 (not a number): infinity, 0 x infinity = NaN
+    auto vscale = [&](uint32_t d, int j) {                                        // byte j << 23; byte 255 (not a number): infinity, 0 x infinity = NaN
+      uint32_t r;
+      switch (j) {
+        case 0: asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(d)); break;
+        case 1: asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(d)); break;
+        case 2: asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(d)); break;
+        default: asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(d));
+      }
+      return __uint_as_float(r);
+    };
     auto value = [&](int i) {                                                     // operand of dims 16 i + col
       const uint32_t d = i < 4 ? f.v0[i & 3] : f.v1[i & 3];
       union { bf16x2 h[4]; bf16x8 v; } u;
@@ -244,7 +256,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       hide(vs0, vs1);
       float y[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = ((var & 1) ? lo[j] : hi[j]) * vscale(j < 4 ? vs0 : vs1, j & 3);
+      for (int j = 0; j < 8; ++j) y[j] = hi[j] * vscale(j < 4 ? vs0 : vs1, j & 3);
       B b;
 #pragma unroll
       for (int j = 0; j < 4; ++j) b.d[j] = pack(y[2 * j], y[2 * j + 1]);
@@ -262,10 +274,6 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) { const bf16x8 v = value(i); acc[i] = MFMA16(v, bh.v, acc[i]); acc[i] = MFMA16(v, bl.v, acc[i]); }
     } else {
-      if constexpr (MODE == 3) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) hi[j] = var ? lo[j] : hi[j];
-      }
       auto block = [&](auto BLK) {                                                // four lanes hold the four blocks' scales: taken from the neighbour (quad_perm)
         constexpr int blk = decltype(BLK)::value;
         uint32_t d0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)vs0, blk * 0x55, 0xf, 0xf, true);
@@ -275,7 +283,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float s0 = vscale(j < 2 ? d0 : d1, 2 * j & 3), s1 = vscale(j < 2 ? d0 : d1, (2 * j + 1) & 3);
-          bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);                     // MODE 3: hi is the half that this column holds
+          bh.d[j] = pack(hi[2 * j] * s0, hi[2 * j + 1] * s1);
           if constexpr (MODE == 2) bl.d[j] = pack(lo[2 * j] * s0, lo[2 * j + 1] * s1);
         }
 #pragma unroll
@@ -342,7 +350,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
 }
 
 template <int D, int MODE, int NW, bool ALIBI>
-__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 1) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
 
 // beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once,
 // in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: 45.6 us, 49.0 as MODE 2)
