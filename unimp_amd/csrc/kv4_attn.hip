@@ -112,18 +112,20 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   // every lane's loads of page k, unconditional (past the last page: that one again, from the cache), so that the number in flight is known everywhere
   auto load = [&](Kv4Frag<D>& f, int k) {
     const uint8_t* page = page_of(min(k, n - 1));
+    uint32_t k_off = k_at, ks_off = ks_at, v_off = v_at, vs_off = vs_at;          // 32-bit offsets of this block: the page's address stays scalar
+    asm volatile("" : "+v"(k_off), "+v"(ks_off), "+v"(v_off), "+v"(vs_off));
     typedef __attribute__((ext_vector_type(4), aligned(8))) uint32_t u32x4h;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) f.k[h] = *(const u32x4h*)(page + k_at + k_step * h);
-    f.ks = *(const uint16_t*)(page + ks_at);
+    for (int h = 0; h < 2; ++h) f.k[h] = *(const u32x4h*)(D == 80 ? page + (k_off + k_step * h) : page + k_off + 256 * h);
+    f.ks = *(const uint16_t*)(page + ks_off);
     if constexpr (D == 80) {
       typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4u;
-      f.v0 = *(const u32x4u*)(page + v_at); f.v1[0] = *(const uint32_t*)(page + v_at + 16);
+      f.v0 = *(const u32x4u*)(page + v_off); f.v1[0] = *(const uint32_t*)(page + v_off + 16);
     } else {
-      f.v0 = *(const u32x4*)(page + v_at);
-      if (D == 128) f.v1 = *(const u32x4*)(page + v_at + 16);
+      f.v0 = *(const u32x4*)(page + v_off);
+      if (D == 128) f.v1 = *(const u32x4*)(page + v_off + 16);
     }
-    f.vs = *(const u32x2*)(page + vs_at);                                        // of the lane's block; MODE 2: of block col & 3
+    f.vs = *(const u32x2*)(page + vs_off);                                        // of the lane's block; MODE 2: of block col & 3
   };
 
   Kv4Frag<D> fa, fb;
