@@ -12,9 +12,9 @@
 //            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
 //            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 3: (query, half) columns, a product per block;
 //            MODE 2: 16 queries, block and half as products.  Measured, 64 rows x 8 key heads x 128 dims of up to 8 000 tokens (all of 8 000), TB/s of pages: MODE 0 (1 or 2 queries
-//            of a key head) 5.0 (5.7), MODE 1 (4) 4.8 (5.5), MODE 3 (8) 4.2 (5.0; as MODE 2 it was 3.9 (4.6)), MODE 2 (16) 3.7 (4.3).
-// Bound by the bytes of the pages, 17 / 32 of a byte per element, where there are many (a large read reaches 5.75 TB/s here; the matrix pipe is a sixth busy), else by the chain
-// length -> page id -> page -> join: one row of 469 tokens x 32 heads x 80 7.2 us, ten rows 8.9.
+//            of a key head) 5.4 (6.0), MODE 1 (4) 5.1 (5.8), MODE 3 (8) 4.6 (5.4), MODE 2 (16) 4.0 (4.6); before its other steps MODE 3 read 4.2 (5.0) where MODE 2 read 3.9 (4.6).
+// Bound by the bytes of the pages, 17 / 32 of a byte per element, where there are many (a large read by torch reaches 5.75 TB/s here, this 6.0; the matrix pipe is a sixth busy), else by the chain
+// length -> page id -> page -> join: one row of 469 tokens x 32 heads x 80 6.6 us, ten rows 8.1.
 #include <type_traits>
 #include "kv4.h"
 #include "unimp_hip.h"
@@ -356,7 +356,7 @@ template <int D, int MODE, int NW, bool ALIBI>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 1) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
 
 // beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once,
-// in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: 45.6 us, 49.0 as MODE 2)
+// in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: 41.7 us; 45.6 before its other steps where MODE 2 took 49.0)
 template <int D, int MODE, int GMODE, bool ALIBI>
 __global__ __launch_bounds__(256) void kv4_attn_group_kernel(Kv4AttnArgs a) {
   if ((int)blockIdx.z >= (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) kv4_attn_part<D, GMODE, 4, 1, ALIBI, true>(a);
@@ -420,17 +420,16 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   const int G = d->heads / d->kv_heads;
   const long units = (long)d->rows * d->kv_heads;
   p.mode = mode(G);
-  // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads, pages = rows x heads x columns: 10 beams x 80, prompt
-  // 469 (5 120 pages) 12.7 | 9.2, 1 024 (10 560) 13.1 | 15.2, 4 096 17.4 | 27.9; 40 rows, prompt 128 (6 400) 11.6 | 10.3, 469 (20 480) 14.9 | 18.2, 4 096 34.5 | 75.1
+  // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads x 80, pages = rows x heads x columns: 10 beams, prompt 469
+  // (5 120 pages) 10.7 | 7.5, 1 024 (10 560) 10.6 | 10.3, 4 096 (41 280) 15.6 | 22.0; 40 rows, prompt 128 (6 400) 10.4 | 7.9, 469 (20 480) 12.6 | 15.1, 4 096 28.9 | 60.7
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
   p.gmode = mode(p.group * G);
-  // waves of a workgroup: eight where a row is one chunk and workgroups are few -- up to 256 pairs, and up to 512 of head dim 64 and 80, whose registers let two such workgroups share a
-  // CU (512 pairs x 80 dims of up to 2 048 tokens: four waves 17.0 us, eight 15.6, all of 2 048 19.7 | 19.2; of 128 dims 17.2 | 19.4); one where rows are short and many
-  const bool few = units <= 256 ? d->width <= (units > 64 ? 48 : 32) : units <= 512 && d->hd < 128 && d->width > 40 && d->width <= 64;
-  p.nw = p.mode >= 2 || p.group > 1 ? 4 : few ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
-  // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 66.7 us, 48 61.6, 64 67.4, 96 61.8).
-  // Fewer: one chunk where a wave has few pages then (no merge: 8 query heads to a key head, 20 pages: 9.5 -> 8.4 us; 128 pairs x 47 pages, eight waves: 11.8 -> 10.2), else as many
-  // as make 512 workgroups of at least 16 pages (128 pairs x 157 pages: 4 chunks 17.2 us, 5 18.8, 8 20.6; 256 x 50: 2 chunks 13.0, 3 15.5; 32 x 63: 4 chunks 9.1, 2 11.4)
+  // waves of a workgroup: eight where a row is one chunk and workgroups are few (128 pairs x 47 pages 8.5 us, two chunks of four waves 10.5; 512 pairs x 128 dims of up to 2 048 tokens:
+  // four waves 15.8, eight 17.8), one where rows are short and many
+  p.nw = p.mode >= 2 || p.group > 1 ? 4 : units <= 256 && d->width <= (units > 64 ? 48 : 32) ? 8 : units >= 1024 && d->width <= 16 ? 1 : 4;
+  // 512 (row, key head) pairs and more: whole rows up to 2 048 tokens, 48 pages above (64 rows x 8 key heads of up to 8 000 tokens: 32 pages 52.1 us, 48 48.1, 64 53.9, 96 49.7).
+  // Fewer: one chunk where a wave has few pages then (no merge: 8 query heads to a key head, 20 pages: 9.3 -> 8.2 us), else as many as make 512 workgroups of at least 16 pages
+  // (128 pairs x 157 pages: 4 chunks 14.6 us, 5 16.6, 8 16.5; 256 x 50: 2 chunks 12.1, 3 13.4; 32 x 63: 4 chunks 8.1, 2 10.0)
   const int most = d->width <= 64 ? 64 : 48, least = p.nw == 8 ? 64 : d->width <= 32 ? 32 : 16, parts = units < 512 ? (int)(512 / (units > 0 ? units : 1)) : 1;
   p.chunk = clamp((d->width + parts - 1) / parts, least, most);
   p.chunk_p = p.slots_p = 0;
