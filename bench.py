@@ -648,7 +648,7 @@ def main():
         dist.init_process_group(backend, init_method=f"tcp://127.0.0.1:{port_}", rank=0, world_size=1,
                                 **({"device_id": dev} if backend == "nccl" else {}))
 
-    from unimp_amd import ops
+    from unimp_amd import hostcomm, ops
     from unimp_amd import functional as F_
     from unimp_amd.synthetic import make_batch
     from unimp_amd.train import Trainer
@@ -721,8 +721,8 @@ def main():
     if prof is None:
         prof, ops.GEMM_PROFILE = ops.GEMM_PROFILE, None
     if world > 1:
-        t = torch.tensor([dt], device=dev if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        t = torch.tensor([dt], device=dev, dtype=torch.float64)
+        hostcomm.all_reduce(t, dist.ReduceOp.MAX, None)
         dt = t.item()
     ms = dt / args.steps * 1e3
     value = GA * B * world * args.steps / dt          # mmrec.py:267-272: GA x batch x world / step time
@@ -749,8 +749,8 @@ def main():
             torch.cuda.synchronize()
             dtp = time.perf_counter() - tp0
             if world > 1:
-                t = torch.tensor([dtp], device=dev if dist.get_backend() == "nccl" else "cpu", dtype=torch.float64)
-                dist.all_reduce(t, op=dist.ReduceOp.MAX)
+                t = torch.tensor([dtp], device=dev, dtype=torch.float64)
+                hostcomm.all_reduce(t, dist.ReduceOp.MAX, None)
                 dtp = t.item()
             packed_leg = {"value": round(B * world * kp / dtp, 3), "unit": "samples/s", "ms_per_step": round(dtp / kp * 1e3, 2), "steps": kp, "warmup": 4,
                           "loss": float(loss_p), "vs_padded": round(B * world * kp / dtp / value, 4),

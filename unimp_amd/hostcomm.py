@@ -1,12 +1,13 @@
-"""Collectives for a backend that moves host memory (gloo: CPU runs, and several ranks that share one GPU).  A device tensor is staged through host memory with synchronous
-copies: gloo's own device path works on streams of another priority and has hung where several ranks shared a card.  RCCL never comes here."""
+"""Collectives on device tensors whose group hands them to gloo (CPU runs' backend, also of several ranks that share one GPU): staged through host memory with synchronous copies,
+because gloo's own device path works on streams of another priority and has hung where several ranks shared a card.  Every other backend takes the tensor itself."""
 import torch
 import torch.distributed as dist
 
 
 def staged(t, group):
-    """does a collective of ``group`` on ``t`` go through host memory?"""
-    return t.is_cuda and dist.get_backend(group) != "nccl"
+    """does a collective of ``group`` on ``t`` go through host memory?  Decided by the backend that the group has for the tensor's device type: a group's name does not tell it (made
+    without a backend it is "undefined", with one per device type "cpu:gloo,cuda:nccl"; both take device tensors over RCCL)"""
+    return t.is_cuda and "cuda:gloo" in str(dist.get_backend_config(group)).split(",")
 
 
 class _Staged:
