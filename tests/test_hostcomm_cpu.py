@@ -1,4 +1,4 @@
-"""hostcomm without a GPU: which collectives go through host memory."""
+"""hostcomm without a GPU: which collectives go through host memory, and that a staged sum reaches its tensor once."""
 from types import SimpleNamespace
 
 import pytest
@@ -33,3 +33,16 @@ def test_config_of_a_real_group(tmp_path):
         assert torch.equal(out, torch.arange(4.))
     finally:
         dist.destroy_process_group()
+
+
+def test_a_second_wait_changes_nothing(monkeypatch):
+    """the sum is copied over its tensor once: what was written there since stays"""
+    monkeypatch.setattr(dist, "all_reduce", lambda t, op, group, async_op: SimpleNamespace(wait=lambda: None))
+    t = torch.ones(3)
+    h = hostcomm._Staged(t, dist.ReduceOp.SUM, None)
+    h.host = torch.full((3,), 2.)                                   # the sum (a host copy of a host tensor is the tensor itself)
+    h.wait()
+    assert torch.equal(t, torch.full((3,), 2.))
+    t.fill_(5.)                                                     # the next step's gradients
+    h.wait()
+    assert torch.equal(t, torch.full((3,), 5.))

@@ -11,7 +11,7 @@ def staged(t, group):
 
 
 class _Staged:
-    """handle of an asynchronous all-reduce of a host copy; the sum reaches the device tensor in wait()"""
+    """handle of an asynchronous all-reduce of a host copy; the sum reaches the device tensor in the first wait()"""
 
     def __init__(self, t, op, group):
         self.t, self.host = t, t.to("cpu")                    # synchronous: every kernel that writes t has finished
@@ -19,7 +19,9 @@ class _Staged:
 
     def wait(self):
         self.work.wait()
-        self.t.copy_(self.host)
+        if self.t is not None:
+            self.t.copy_(self.host)
+            self.t = None
 
 
 def all_reduce(t, op, group, async_op=False):
