@@ -3,7 +3,9 @@ same (bf16-representable) weights and the same synthetic batch.  TEST INFRASTRUC
 import torch
 
 from oracle import flamingo as ofl, lm as olm, mpt as ompt, vit as ovit, train_step as ots
+import _gloo_host
 
+_gloo_host.install()          # worker processes only: no device tensor goes to gloo
 bf16 = torch.bfloat16
 
 TINY = dict(vit=dict(image_size=32, patch_size=8, width=128, layers=2, heads=2, mlp_dim=256, output_dim=64),

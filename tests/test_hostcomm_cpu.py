@@ -1,9 +1,14 @@
 """hostcomm without a GPU: which collectives go through host memory, and that a staged sum reaches its tensor once."""
+import os
+import sys
 from types import SimpleNamespace
 
 import pytest
 import torch
 import torch.distributed as dist
+import torch.multiprocessing as mp
+
+import _gloo_host
 
 from unimp_amd import hostcomm
 
@@ -46,3 +51,35 @@ def test_a_second_wait_changes_nothing(monkeypatch):
     t.fill_(5.)                                                     # the next step's gradients
     h.wait()
     assert torch.equal(t, torch.full((3,), 5.))
+
+
+def _worker(rank, store, q):
+    sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+    import _parity  # noqa: F401 -- what the GPU tests' workers import before they exchange anything
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2)
+    hostcomm.staged = lambda t, group: t.numel() > 2               # stands for a device tensor
+    seen, wrapped = [], sys.modules["_gloo_host"]
+    wrapped.plain = lambda parts, t, group=None, async_op=False, plain=wrapped.plain: (seen.append(t.numel()), plain(parts, t, group=group, async_op=async_op))[1]
+    got = []
+    for n in (2, 5):
+        t = torch.arange(float(n)) + 10 * rank
+        parts = [torch.full((n,), -1.) for _ in range(2)]
+        dist.all_gather(parts, t)
+        got.append([p.tolist() for p in parts])
+    q.put((rank, got, seen, dist.all_gather is wrapped.all_gather))
+    dist.destroy_process_group()
+
+
+def test_workers_gather_through_host_memory(tmp_path):
+    assert dist.all_gather is _gloo_host.plain                     # not in a program of its own
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_worker, args=(r, str(tmp_path / "store"), q)) for r in range(2)]
+    for p in ps:
+        p.start()
+    res = sorted(q.get(timeout=120) for _ in ps)
+    for p in ps:
+        p.join(60)
+    for rank, got, seen, wrapped in res:
+        assert wrapped and seen == [2, 5]
+        assert got == [[[0., 1.], [10., 11.]], [[float(i) for i in range(5)], [10. + i for i in range(5)]]]
