@@ -441,7 +441,7 @@ int unimp_image_resize_normalize(const uint8_t* src, const unimp_image_desc* des
 
 /* ---- paged K/V cache held in 4 bits (decode; eval_rec.py:100-110, eval_exp.py:103-113, eval_img_gen.py:102-111 through Flamingo.generate) -----
  * A page holds 32 tokens of one head of one layer, keys and values, as MX blocks: e2m1 codes with one E8M0 scale byte per (token, 32 consecutive dims; the
- * last block of a head dim of 80 is 16 wide): 2^e, e = max(floor(log2 of the block's largest magnitude) - 2, -125), codes rounded to nearest even, saturated at
+ * last block of a head dim of 80 is 16 wide): 2^e, e = floor(log2 of the block's largest magnitude) - 2, at least -125 and at most 125, codes rounded to nearest even, saturated at
  * 6; a block that holds an infinity or a NaN is stored as scale 255 and reads back as NaN.  unimp_kv4_page_bytes(hd) = 32 hd + 64 ceil(hd / 32) bytes (head dims 64, 80,
  * 128; -1: any other) against 128 hd in bf16.  Byte layout: unimp_amd/csrc/kv4.h.  A pool is [n_pages][heads][page bytes] per layer, 16-byte aligned;
  * SLOT s = token s % 32 of page s / 32.  A row's pages are named by its row of an int32 table: column c = tokens 32 c ... 32 c + 31.

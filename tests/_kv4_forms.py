@@ -104,3 +104,14 @@ def write_pages(before, slots, k, v):
         nib[page, h, where], nib[page, h, where + 1] = (scales & 15).to(torch.uint8), (scales >> 4).to(torch.uint8)
     nib = nib.view(n_pages, heads, nbytes, 2)
     return nib[..., 0] | nib[..., 1] << 4
+
+
+def rotated(x, cos, sin, rot):
+    """x [rows, heads, hd] float64, half-split pairs of the first rot dims turned by the rows' fp32 tables"""
+    c, s, h = cos.double()[:, None], sin.double()[:, None], rot // 2
+    return torch.cat([x[..., :h] * c - x[..., h:rot] * s, x[..., h:rot] * c + x[..., :h] * s, x[..., rot:]], -1)
+
+
+def saturated(x):
+    """values outside bf16's range, which only a rotation makes: their block's exponent stays 125, codes saturate at 6"""
+    return x.clamp(-6 * 2.0 ** 125, 6 * 2.0 ** 125)

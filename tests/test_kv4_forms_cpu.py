@@ -36,3 +36,12 @@ def test_expected_pages(hd):
             for h in range(2):
                 R.put(want[s // 32, h], s % 32, k[i, h], v[i, h])
     assert torch.equal(F.write_pages(before, slots, k, v), want)
+
+
+def test_what_is_held_is_finite_in_bf16():
+    """two bf16 near the largest value, turned by 45 degrees, are beyond bf16: their block's scale stays one whose codes are values of bf16"""
+    x = torch.full((1, 1, 64), 3e38, dtype=torch.bfloat16).double()
+    y = F.rotated(x, torch.full((1, 32), 0.5 ** 0.5), torch.full((1, 32), 0.5 ** 0.5), 64)
+    assert y.abs().max() > torch.finfo(torch.bfloat16).max and R.quantise(y)[1].max() == 253
+    held = R.held(F.saturated(y))
+    assert torch.equal(held.to(torch.bfloat16).double(), held) and R.quantise(F.saturated(y))[1].max() == 252

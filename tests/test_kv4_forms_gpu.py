@@ -1,4 +1,4 @@
-"""The 4-bit page cache's kernels in every form that their launch rules choose and at the precision that they claim; 64-bit results and bounds in
+"""The 4-bit page cache's kernels in every form that their launch rules choose, at the precision that they claim, and at the ends of the value range; 64-bit results and bounds in
 tests/_kv4_forms.py (tests/test_kv4_forms_cpu.py shows that a p of one bf16 leaves them)."""
 import pytest
 import torch
@@ -112,3 +112,25 @@ def test_long_shared_chunks(ops, hd, K, groups, kvh, G, width):
     args = q.cuda(), pages.cuda(), tables.cuda(), lens.cuda(), hd ** -0.5
     check(ops.kv4_attn_decode(*args, group=K, shared_len=shared.cuda()), want, bound)
     check(ops.kv4_attn_decode(*args), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------- the ends of the value range
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_append_beyond_bf16(ops, hd):
+    """a rotation may take two bf16 beyond bf16's largest value: such a block saturates, what is read back is finite, and the other blocks and rows are those of any append"""
+    rows, heads, rot = 4, 2, hd
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(rows, 3, heads, hd, generator=g).to(bf16)
+    qkv[0, 1] = 3e38
+    qkv[1, 1, 1, :16] = 3e38                                        # pairs of one large and one small value
+    qkv[2, 1, 0, 3], qkv[2, 1, 0, 3 + rot // 2] = 3.3e38, -3.3e38
+    cos, sin = (torch.full((rows, rot // 2), 0.5 ** 0.5) for _ in range(2))
+    slots = torch.tensor([0, 33, 5, 40])
+    pages = torch.zeros((2, heads, R.page_bytes(hd)), dtype=torch.uint8, device="cuda")
+    ops.kv4_rope_append(qkv.view(rows, -1).cuda(), heads, hd, hd, (0, heads * hd, 2 * heads * hd), rot, cos.cuda(), sin.cuda(), pages, slots.cuda())
+    k, v = (x.cpu().double() for x in ops.kv4_read(pages, slots.cuda(), hd))
+    turned = F.rotated(qkv[:, 1].double(), cos, sin, rot)
+    assert turned.abs().max() > torch.finfo(bf16).max
+    lost = int((~torch.isfinite(k)).sum())
+    assert lost == 0
+    assert torch.equal(k, R.held(F.saturated(turned))) and torch.equal(v, R.held(qkv[:, 2]))

@@ -2,7 +2,7 @@
 // quantise-and-write of prompt tokens, rotary embedding + append of a decode step's tokens, read-back as values, page tables and slots from the rows' lengths,
 // and the beam reorder.  Layout of a page: kv4.h.  Attention over the pages: kv4_attn.hip.
 //
-// An MX block of x: e = max(floor(log2 max |x|) - 2, -125), codes rne(x / 2^e) on e2m1, saturated at 6: 2^e code is exact in bf16, so what is read back is
+// An MX block of x: e = floor(log2 max |x|) - 2 between -125 and 125, codes rne(x / 2^e) on e2m1, saturated at 6: 2^e code is exact in bf16, so what is read back is
 // exactly what the attention multiplies.  All of these are bound by bytes; the arithmetic is a few instructions per element.
 #include <type_traits>
 #include "kv4.h"
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const bf16* __rest
     int e = max((int)((__double2hiint(x[0]) >> 20) & 0x7ff), (int)((__double2hiint(x[1]) >> 20) & 0x7ff));
     e = max(e, kv4_dpp<0xB1>(e)); e = max(e, kv4_dpp<0x4E>(e));     // lane ^ 1, ^ 2: quads agree
     e = max(e, kv4_dpp<0x141>(e)); e = max(e, kv4_dpp<0x140>(e));   // mirrored inside 8 and inside 16 lanes
-    sb[w] = e == 2047 ? 255 : max(e - 1023 - 2, -125) + 127;
+    sb[w] = e == 2047 ? 255 : min(max(e - 1023 - 2, -125), 125) + 127;      // a rotation may leave bf16's range: saturated like any code above 6
     const double inv = __hiloint2double((1023 + 127 - sb[w]) << 20, 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) code[w][j] = sb[w] == 255 ? 0u : kv4_code_f64(x[j], inv);
