@@ -134,3 +134,43 @@ def test_append_beyond_bf16(ops, hd):
     lost = int((~torch.isfinite(k)).sum())
     assert lost == 0
     assert torch.equal(k, R.held(F.saturated(turned))) and torch.equal(v, R.held(qkv[:, 2]))
+
+
+@pytest.mark.parametrize("G", [1, 4, 8, 16])
+@pytest.mark.parametrize("hd,power", [(64, 125), (80, 125), (128, 125), (64, -74), (80, -74), (128, -74)])
+def test_values_of_any_magnitude(ops, hd, power, G):
+    """values up to bf16's largest and down to 2^-74: no sum of p v leaves 32 bits, whether scores rise along the row (the maximum lags behind them), are all alike or fall"""
+    kvh, W = 2, 100
+    g = torch.Generator().manual_seed(hd + G)
+    k = torch.randn(2 * W, kvh, 32, hd, generator=g).to(bf16)
+    v = torch.randn(2 * W, kvh, 32, hd, generator=g).clamp(-3.9, 3.9)
+    v[W:] = v[W:].abs()                                             # the second row's values do not cancel
+    pages = R.pack(k, (v.double() * 2.0 ** power).to(bf16))
+    tables = torch.arange(2 * W, dtype=torch.int32).view(2, W)
+    lens = torch.tensor([3200, 3111], dtype=torch.int32)
+    q = (0.5 * torch.randn(2, kvh * G, hd, generator=g)).to(bf16)
+    rise = torch.full((kvh * G,), 0.02)
+    for slopes in (None, rise, -rise / 8):
+        want, bound, _ = F.attend(q, pages, tables, lens, hd ** -0.5, slopes)
+        check(ops.kv4_attn_decode(q.cuda(), pages.cuda(), tables.cuda(), lens.cuda(), hd ** -0.5, alibi=None if slopes is None else slopes.cuda()), want, bound,
+              "alike" if slopes is None else slopes[0].item())
+
+
+@pytest.mark.parametrize("hd,K,groups,kvh,G,width", [F.GROUPS[0], F.GROUPS[1], F.GROUPS[2], F.GROUPS[5]])
+@pytest.mark.parametrize("power", [125, -74])
+def test_values_of_any_magnitude_in_groups(ops, hd, K, groups, kvh, G, width, power):
+    g = torch.Generator().manual_seed(hd + G)
+    rows = K * groups
+    v = torch.randn(30, kvh, 32, hd, generator=g).clamp(-3.9, 3.9).abs()
+    pages = R.pack(torch.randn(30, kvh, 32, hd, generator=g).to(bf16), (v.double() * 2.0 ** power).to(bf16))
+    tables = torch.full((rows, width), -1, dtype=torch.int32)
+    tables[:, :12] = torch.arange(12, dtype=torch.int32)
+    tables[:, 12] = torch.randint(12, 30, (rows,), generator=g).to(torch.int32)
+    lens = torch.tensor([385 + r % 32 for r in range(rows)], dtype=torch.int32)
+    q = (0.5 * torch.randn(rows, kvh * G, hd, generator=g)).to(bf16)
+    shared = torch.full((groups,), 384, dtype=torch.int32)
+    rise = torch.full((kvh * G,), 0.02)
+    for slopes in (None, rise):
+        want, bound, _ = F.attend(q, pages, tables, lens, hd ** -0.5, slopes)
+        check(ops.kv4_attn_decode(q.cuda(), pages.cuda(), tables.cuda(), lens.cuda(), hd ** -0.5, alibi=None if slopes is None else slopes.cuda(), group=K, shared_len=shared.cuda()),
+              want, bound, slopes is None)

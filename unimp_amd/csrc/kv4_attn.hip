@@ -5,8 +5,10 @@
 //   scores   S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4: A = the page's K codes and scale bytes AS STORED (kv4.h: a lane's operand is one 16-byte load),
 //            B = the queries in its 16 columns, each 32-dim block of a query as e4m3 hi + lo under a shared power-of-two scale.  A bf16 has 8 significant bits, e4m3 four:
 //            hi + lo is exact for elements down to 2^-10 of the block's largest and within 2^-17 of that one below.
-//   softmax  online, base 2, lane (column c, group g) holds tokens 16 h + 4 g + e of the page; the running maximum moves only when a score exceeds it by 2^10 (p <= 1024
-//            costs nothing in fp32), so the common page has no cross-lane step and no rescale.
+//   softmax  online, base 2, lane (column c, group g) holds tokens 16 h + 4 g + e of the page; the running reference point m lies 8 above the maximum when it moves, and moves
+//            only when a score exceeds it by 2 (p <= 4), so the common page has no cross-lane step and no rescale.
+//   range    p times V's scale and its sums stay in fp32 for every value that a page holds: p <= 2^2, scale <= 2^125, and V's codes enter the product times 2^-24 (the last division takes it
+//            back), so 2^21 tokens (the widest table) of 6 2^125 make less than 2^127.  Downwards a p V below 2^-94 is subnormal there.
 //   o^T     += V^T P^T on v_mfma_f32_16x16x32_bf16: A = V's nibbles through v_cvt_scalef32_pk_bf16_fp4 (exact), B = p times the token's V scale, which differs per 32 dims.
 //            p is split in two bf16 (16 bits kept).  The scale blocks and the two halves are COLUMNS of B where the queries leave room: with one or two queries
 //            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
@@ -21,6 +23,9 @@
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 #define KV4_TEAMS 4                    // rows of a workgroup on a beam group's tails
+#define KV4_AHEAD 8.f                  // log2: how far m is set above the maximum; p of the largest score is 2^-8 ... 2^2
+#define KV4_LAG 2.f                    // log2: how far a score may exceed m
+#define KV4_V_UNIT 0x1p-24f            // V's codes in the product; sums carry it to the end
 
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
@@ -39,7 +44,7 @@ template <int D> struct Kv4Frag {        // one page as a wave holds it
   u32x4 k[2]; u32x4 v0; u32x4 v1; uint32_t ks; u32x2 vs;
 };
 
-// slot i of a (row, head) in the workspace: [0, slots_p) the group's columns, then the row's own; hd sums, maximum, sum of exponentials
+// slot i of a (row, head) in the workspace: [0, slots_p) the group's columns, then the row's own; hd sums, reference point, sum of exponentials
 __device__ __forceinline__ float* kv4_partial(const Kv4AttnArgs& a, int D, int row, int head, int slot) {
   return a.ws + (((long)row * a.heads + head) * (a.slots_p + a.slots) + slot) * (D + 2);
 }
@@ -176,7 +181,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
   f32x4 acc[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, mu = 0.f, l = 0.f;                                         // running maximum; the same, 0 while there is none; sum of this lane's tokens
+  float m = -INFINITY, mu = 0.f, l = 0.f;                                         // reference point; the same, 0 while there is none; sum of this lane's tokens
 
   auto compute = [&](const Kv4Frag<D>& f, int k) {
     const int c = c0 + w + NW * k;
@@ -206,10 +211,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       for (int j = 0; j < 8; ++j) if (16 * (j >> 2) + g4 + (j & 3) >= vis) x[j] = -INFINITY;
     }
     const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(mx > m + 10.f)) {
+    if (__any(mx > m + KV4_LAG)) {
       float t = fmaxf(mx, __shfl_xor(mx, 16, 64));
       t = fmaxf(t, __shfl_xor(t, 32, 64));
-      t = fmaxf(t, m);
+      t = fmaxf(t + KV4_AHEAD, m);
       const float r = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - t);
       m = t; mu = t == -INFINITY ? 0.f : t;
       l *= r;
@@ -242,10 +247,10 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
     auto value = [&](int i) {                                                     // operand of dims 16 i + col
       const uint32_t d = i < 4 ? f.v0[i & 3] : f.v1[i & 3];
       union { bf16x2 h[4]; bf16x8 v; } u;
-      u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 0);
-      u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 1);
-      u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 2);
-      u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.f, 3);
+      u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, KV4_V_UNIT, 0);
+      u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, KV4_V_UNIT, 1);
+      u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, KV4_V_UNIT, 2);
+      u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, KV4_V_UNIT, 3);
       return u.v;
     };
     union B { uint32_t d[4]; bf16x8 v; };
@@ -347,7 +352,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       p[d] = o;
       if (d == 0) { p[D] = M; p[D + 1] = L; }
     } else {
-      a.o[r * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : o / L);
+      a.o[r * a.o_rs + h * a.o_hs + d] = f2bf(L == 0.f ? 0.f : o / L * (1.f / KV4_V_UNIT));
     }
   }
 }
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(PARTS * D / 2) void kv4_attn_merge_kernel(Kv4AttnAr
     for (int i = 0; i < PARTS; ++i) { const float e = __builtin_amdgcn_exp2f(sm[i] - u); l = fmaf(sl[i], e, l); o0 = fmaf(so[i][d], e, o0); o1 = fmaf(so[i][d + 1], e, o1); }
   }
   bf16* o = a.o + row * a.o_rs + h * a.o_hs + d;
-  o[0] = f2bf(l == 0.f ? 0.f : o0 / l); o[1] = f2bf(l == 0.f ? 0.f : o1 / l);
+  o[0] = f2bf(l == 0.f ? 0.f : o0 / l * (1.f / KV4_V_UNIT)); o[1] = f2bf(l == 0.f ? 0.f : o1 / l * (1.f / KV4_V_UNIT));
 }
 
 struct Kv4Plan { int mode, gmode, nw, chunk, slots, group, chunk_p, slots_p; int64_t floats; };
