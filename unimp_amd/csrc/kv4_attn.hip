@@ -443,12 +443,8 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
     p.chunk_p = clamp((long)d->width * (units / p.group) / 512, 16, 64);
     p.slots_p = (d->width + p.chunk_p - 1) / p.chunk_p;
   }
-  // longer chunks where a row would have more partials than the merge is made for (over 524 288 tokens at 64 pages)
+  // longer chunks where a row would have more partials than the merge is made for (over 393 216 tokens at 48 pages); groups end at 16 KV4_MAX_SLOTS columns
   if (d->width > (long)KV4_MAX_SLOTS * p.chunk) p.chunk = (d->width + KV4_MAX_SLOTS - 1) / KV4_MAX_SLOTS;
-  if (p.group > 1 && d->width > (long)KV4_MAX_SLOTS * p.chunk_p) {
-    p.chunk_p = (d->width + KV4_MAX_SLOTS - 1) / KV4_MAX_SLOTS;
-    p.slots_p = (d->width + p.chunk_p - 1) / p.chunk_p;
-  }
   p.slots = d->width > 0 ? (d->width + p.chunk - 1) / p.chunk : 1;
   p.floats = p.group == 1 && p.slots == 1 ? 0 : (int64_t)d->rows * d->heads * (p.slots + p.slots_p) * (d->hd + 2);
   return p;
