@@ -452,7 +452,7 @@ int unimp_kv4_page_bytes(int hd);
  * contents in that token, in no other). */
 int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, void* pages, int64_t n_pages, int heads, int hd,
                     const int64_t* slots, int64_t tokens, void* stream);
-/* a decode step's tokens: rotate q and k of every row (half-split pairs, row r with ITS table row; rot = 0: none), write q (bf16, rounded once) to q_out
+/* a decode step's tokens: rotate q and k of every row (half-split pairs, row r with ITS table row; rot = 0: none), write q (bf16, rounded through fp32) to q_out
  * [rows][heads][hd] and quantise the rotated k and v into slot slots[r] (different ones).  Operand layout of unimp_decode_rope_append; qkv is not modified.  The rotation is computed in
  * 64 bits from the fp32 tables. */
 int unimp_kv4_rope_append(const void* qkv, int64_t row_stride, int64_t head_stride, int rows, int heads, int hd, int q_off, int k_off, int v_off, int rot,

@@ -270,7 +270,7 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
   if (!k || !v || !pages || !slots) return unimp_set_error(UNIMP_ERR_ARG, "kv4_write: null pointer");
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
   const int cr = kv4_chunk_rows(tokens, hb);
-  if (heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^31 token heads");
+  if (heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23) return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_write: at most 65535 heads and 2^30 token heads");
   if (((k_ts | k_hs | v_ts | v_hs) & 7) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15))
     return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_write: strides multiples of 8 elements, 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
@@ -281,9 +281,10 @@ extern "C" int unimp_kv4_write(const void* k, const void* v, int64_t k_ts, int64
 }
 
 // ------------------------------------------------------------------------------------------- decode step: rotary embedding + append
-// A wave per (row, head), two dims to a lane.  The rotation runs in 64 bits (two products of a bf16 and an fp32, exact there): a code is decided next to a border, and
-// k's codes are those of the exact rotation of the given tables.  V's nibbles go in by atomics: two rows of a launch may write different tokens of one page.  Bound by its
-// three dependent steps (load, block maximum, write), not by bytes: 10 rows x 32 x 80 4.1 us, 200 x 32 x 128 10 us (7.6 MB).
+// A wave per (row, head), two dims to a lane.  The rotation runs in 64 bits (two products of a bf16 and an fp32, exact there, and their sum): a code is decided next to a border, and
+// k's codes are those of the given tables' rotation in 64 bits.  V's nibbles go in by atomics: two rows of a launch may write different tokens of one page.  A few rows are bound by
+// three dependent steps (load, block maximum, write): 10 rows x 32 x 80 4.1 us.  Many rows are not, nor by bytes: 200 x 32 x 128 10.1 us for 7.6 MB, 258 vector instructions a wave (the
+// codes' comparisons in 64 bits among them) on 6 waves a SIMD beside two atomics a lane.
 __device__ __forceinline__ uint32_t kv4_code_f64(double x, double inv) {
   const double a = fabs(x) * inv;
   const uint32_t c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
@@ -468,7 +469,7 @@ extern "C" int unimp_kv4_read(const void* pages, int64_t layer_stride, int layer
   const int64_t hb = (heads + KV4_HEADS - 1) / KV4_HEADS;
   const int cr = kv4_chunk_rows(tokens, hb * layers);
   if (layers > 65535 || heads > 65535 || (tokens + 31) / 32 * hb > 1 << 23)
-    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^31 token heads");
+    return unimp_set_error(UNIMP_ERR_SHAPE, "kv4_read: at most 65535 layers and heads, 2^30 token heads");
   if (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) return unimp_set_error(UNIMP_ERR_ALIGN, "kv4_read: 16-byte aligned pointers");
   return kv4_for_hd(hd, [&](auto d) {
     constexpr int D = decltype(d)::value;

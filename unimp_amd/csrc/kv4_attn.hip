@@ -14,8 +14,8 @@
 //            (MODE 0) every column is another (query, block, half) and a lane prepares 8 values per page instead of 64; the tile of dims 16 i ... takes the
 //            columns of its block and ignores the others.  MODE 1: (query, block) columns, the halves as two products; MODE 3: (query, half) columns, a product per block;
 //            MODE 2: 16 queries, block and half as products.  Measured, 64 rows x 8 key heads x 128 dims of up to 8 000 tokens (all of 8 000), TB/s of pages: MODE 0 (1 or 2 queries
-//            of a key head) 5.4 (6.0), MODE 1 (4) 5.1 (5.8), MODE 3 (8) 4.6 (5.4), MODE 2 (16) 4.0 (4.6); before its other steps MODE 3 read 4.2 (5.0) where MODE 2 read 3.9 (4.6).
-// Bound by the bytes of the pages, 17 / 32 of a byte per element, where there are many (a large read by torch reaches 5.75 TB/s here, this 6.0; the matrix pipe is a sixth busy), else by the chain
+//            of a key head) 5.7 (5.5), MODE 1 (4) 5.5 (5.1), MODE 3 (8) 4.9 (4.9), where MODE 2 reads 4.5 (4.85), MODE 2 (16) 4.1 (4.6).
+// Bound by the bytes of the pages, 17 / 32 of a byte per element, where there are many (a large read by torch reaches 5.75 TB/s here, this 5.7; the matrix pipe is a sixth busy), else by the chain
 // length -> page id -> page -> join: one row of 469 tokens x 32 heads x 80 6.6 us, ten rows 8.1.
 #include <type_traits>
 #include "kv4.h"
@@ -361,7 +361,7 @@ template <int D, int MODE, int NW, bool ALIBI>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 1) void kv4_attn_kernel(Kv4AttnArgs a) { kv4_attn_part<D, MODE, NW, 1, ALIBI, false>(a); }
 
 // beam groups: the first workgroups (z) take the rows' own columns, few pages each: a wave per row; the others a group's shared columns for up to 16 queries at once,
-// in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: 41.7 us; 45.6 before its other steps where MODE 2 took 49.0)
+// in the mode that their number allows (GMODE; 8 prompts x 5 beams x 32 heads x 128 behind 4 096 shared tokens: MODE 3 41.7 us, MODE 2 44.3)
 template <int D, int MODE, int GMODE, bool ALIBI>
 __global__ __launch_bounds__(256) void kv4_attn_group_kernel(Kv4AttnArgs a) {
   if ((int)blockIdx.z >= (a.rows + KV4_TEAMS - 1) / KV4_TEAMS) kv4_attn_part<D, GMODE, 4, 1, ALIBI, true>(a);
@@ -426,7 +426,9 @@ static Kv4Plan kv4_plan(const unimp_kv4_attn_desc* d) {
   const long units = (long)d->rows * d->kv_heads;
   p.mode = mode(G);
   // groups cost a merge and pay by reading the shared columns once.  Measured (us, groups | every row for itself), 32 heads x 80, pages = rows x heads x columns: 10 beams, prompt 469
-  // (5 120 pages) 10.7 | 7.5, 1 024 (10 560) 10.6 | 10.3, 4 096 (41 280) 15.6 | 22.0; 40 rows, prompt 128 (6 400) 10.4 | 7.9, 469 (20 480) 12.6 | 15.1, 4 096 28.9 | 60.7
+  // (5 120 pages) 10.6 | 7.4, 800 (8 320) 10.5 | 9.0, 1 024 (10 560) 10.7 | 10.0, 1 300 (13 440) 11.0 | 11.3, 4 096 (41 280) 15.4 | 21.6; 40 rows, prompt 128 (6 400) 10.3 | 7.8,
+  // 300 (14 080) 11.7 | 11.5, 469 (20 480) 12.5 | 14.8, 4 096 28.8 | 58.1; 128 dims, 8 x 5 beams, prompt 1 024 (42 240) 20.6 | 21.4, 4 096 41.8 | 67.5.  The two sides meet between 13 000 and
+  // 20 000 pages; from 8 192 up to there a group costs up to 1.5 us, with 4 query heads to a key head 6 (8 x 4 beams x 8 key heads x 128, prompt 1 024, 8 448 pages: 14.2 | 8.1)
   p.group = d->group > 1 && d->shared_len && d->rows % d->group == 0 && d->group * G <= 16 && d->width <= 16 * KV4_MAX_SLOTS && d->width * units >= 8192 ? d->group : 1;
   p.gmode = mode(p.group * G);
   // waves of a workgroup: eight where a row is one chunk and workgroups are few (128 pairs x 47 pages 8.5 us, two chunks of four waves 10.5; 512 pairs x 128 dims of up to 2 048 tokens:
