@@ -5,9 +5,9 @@
 //   scores   S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4: A = the page's K codes and scale bytes AS STORED (kv4.h: a lane's operand is one 16-byte load),
 //            B = the queries in its 16 columns, each 32-dim block of a query as e4m3 hi + lo under a shared power-of-two scale.  A bf16 has 8 significant bits, e4m3 four:
 //            hi + lo is exact for elements down to 2^-10 of the block's largest and within 2^-17 of that one below.
-//   softmax  online, base 2, lane (column c, group g) holds tokens 16 h + 4 g + e of the page; the running reference point m lies 8 above the maximum when it moves, and moves
-//            only when a score exceeds it by 2 (p <= 4), so the common page has no cross-lane step and no rescale.
-//   range    p times V's scale and its sums stay in fp32 for every value that a page holds: p <= 2^2, scale <= 2^125, and V's codes enter the product times 2^-24 (the last division takes it
+//   softmax  online, base 2, lane (column c, group g) holds tokens 16 h + 4 g + e of the page; the running reference point m lies 10 above the maximum when it moves, and moves
+//            only when a score exceeds it (p of the largest score is 2^-10 ... 1), so the common page has no cross-lane step and no rescale.
+//   range    p times V's scale and its sums stay in fp32 for every value that a page holds: p <= 1, scale <= 2^125, and V's codes enter the product times 2^-22 (the last division takes it
 //            back), so 2^21 tokens (the widest table) of 6 2^125 make less than 2^127.  Downwards a p V below 2^-94 is subnormal there.
 //   o^T     += V^T P^T on v_mfma_f32_16x16x32_bf16: A = V's nibbles through v_cvt_scalef32_pk_bf16_fp4 (exact), B = p times the token's V scale, which differs per 32 dims.
 //            p is split in two bf16 (16 bits kept).  The scale blocks and the two halves are COLUMNS of B where the queries leave room: with one or two queries
@@ -23,9 +23,8 @@
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 #define KV4_TEAMS 4                    // rows of a workgroup on a beam group's tails
-#define KV4_AHEAD 8.f                  // log2: how far m is set above the maximum; p of the largest score is 2^-8 ... 2^2
-#define KV4_LAG 2.f                    // log2: how far a score may exceed m
-#define KV4_V_UNIT 0x1p-24f            // V's codes in the product; sums carry it to the end
+#define KV4_AHEAD 10.f                 // log2: how far m is set above the maximum
+#define KV4_V_UNIT 0x1p-22f            // V's codes in the product; sums carry it to the end
 
 struct Kv4AttnArgs {
   const bf16* q; long q_rs, q_hs; const uint8_t* pages; long n_pages; int kv_heads; const int32_t* tables; long t_stride; int width; const int32_t* lens;
@@ -211,7 +210,7 @@ __device__ __forceinline__ void kv4_attn_part(const Kv4AttnArgs& a) {
       for (int j = 0; j < 8; ++j) if (16 * (j >> 2) + g4 + (j & 3) >= vis) x[j] = -INFINITY;
     }
     const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(mx > m + KV4_LAG)) {
+    if (__any(mx > m)) {
       float t = fmaxf(mx, __shfl_xor(mx, 16, 64));
       t = fmaxf(t, __shfl_xor(t, 32, 64));
       t = fmaxf(t + KV4_AHEAD, m);
